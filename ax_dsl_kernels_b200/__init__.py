@@ -9,9 +9,12 @@ from ._lib import Q35Error, device_status, io_table, roles, run, workspace_bytes
 from .attention import (kv_write, mrope_cos_sin, paged_attention_decode, paged_attention_prefill,  # noqa: F401
                         rope_cos_sin)
 from .gdn import gdn_chunk_prefill, gdn_conv1d_silu, gdn_recurrent_step  # noqa: F401
+from .long_context import (evict_keys, page_key_bounds, paged_attention_sparse, paged_key_mass,  # noqa: F401
+                           select_pages)
 from .moe import (linear, moe_block, moe_combine, moe_experts, moe_permute, moe_pre, moe_slots_px,  # noqa: F401
                   prepare_moe_weights, qwen3_moe, route, tile_scales)
 
 __all__ = ["run", "roles", "io_table", "workspace_bytes", "device_status", "Q35Error", "route", "moe_pre",
            "moe_experts", "moe_slots_px", "moe_combine", "moe_permute", "moe_block", "qwen3_moe", "prepare_moe_weights", "tile_scales", "linear",
-           "paged_attention_decode", "paged_attention_prefill", "kv_write", "gdn_recurrent_step", "gdn_conv1d_silu", "gdn_chunk_prefill"]
+           "paged_attention_decode", "paged_attention_prefill", "kv_write", "gdn_recurrent_step", "gdn_conv1d_silu", "gdn_chunk_prefill",
+           "page_key_bounds", "select_pages", "paged_attention_sparse", "paged_key_mass", "evict_keys"]

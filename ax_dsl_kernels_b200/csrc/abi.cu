@@ -191,6 +191,21 @@ static const RoleDef kRoles[] = {
     {"attn.paged_prefill",
      R"({"in":[["q","bf16","[T,HQ,D]"],["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]"],["qo_indptr","i32","[B+1]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["sm_scale","f32","[1] optional"],["kv_scale","f32","[2,HKV] optional: FP8 cache with per-head scales; absent: the stored x 8 form"],["paged_kv_scale","bf16","[pages,2,P,HKV] optional: int8 cache bound as bytes, one scale per row and head; new rows' scales are written"],["k_new","bf16","[T,HKV,D] optional: written into the cache first"],["v_new","bf16","[T,HKV,D] optional"]],"out":[["out","bf16","[T,HQ,D]"]]})",
      run_attn_paged_prefill},
+    {"attn.page_bounds",
+     R"({"in":[["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["first_page","i32","[B] optional: only the sequence's pages from this one on"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes"]],"out":[["page_bounds","bf16","[pages,2,HKV,D]: per channel the minimum and the maximum of the page's keys, E4M3: of the stored codes; pages not listed stay as they were"]]})",
+     run_attn_page_bounds},
+    {"attn.select_pages",
+     R"({"in":[["q","bf16","[B,HQ,D]"],["page_bounds","bf16","[pages,2,HKV,D]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["keep","i32","[2] optional: this many first and last pages are chosen whatever they score"],["workspace","u8","[*]"]],"out":[["pages","i32","[B,HKV,S]: positions in the sequence's page list, ascending, -1 behind"]]})",
+     run_attn_select_pages},
+    {"attn.sparse_decode",
+     R"({"in":[["q","bf16","[B,HQ,D]"],["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["pages","i32","[B,HKV,S] optional: attend to these pages of the sequence only; ascending, -1 behind"],["sm_scale","f32","[1] optional"],["kv_scale","f32","[2,HKV] optional"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes"],["k_new","bf16","[B,HKV,D] optional"],["v_new","bf16","[B,HKV,D] optional"],["cache_location","i32","[B,2] with k_new and key_mass: where the current token's own weight is stored"],["workspace","u8","[*] with key_mass"]],"out":[["out","bf16","[B,HQ,D]"],["key_mass","f32","[pages,P,HKV] optional: the softmax weights of the attended rows, summed over the query heads of a KV head, are added"]]})",
+     run_attn_sparse_decode},
+    {"attn.key_mass",
+     R"({"in":[["q","bf16","[T,HQ,D]"],["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]"],["qo_indptr","i32","[B+1]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["sm_scale","f32","[1] optional"],["kv_scale","f32","[2,HKV] optional"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes"],["accumulate","i32","[1] optional: bound = add to key_mass instead of storing"],["workspace","u8","[*]"]],"out":[["key_mass","f32","[pages,P,HKV]: the weight the window's queries give to every cached row, causal, summed over queries and the query heads of a KV head"]]})",
+     run_attn_key_mass},
+    {"attn.evict",
+     R"({"in":[["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["keep","i32","[2] optional: this many first and last rows stay whatever their weight"]],"out":[["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]: kept rows are moved to the sequence's first K"],["key_mass","f32","[pages,P,HKV]: moves with them"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes: moves with them"],["kept","i32","[B,HKV,K]: the kept rows' old positions, ascending, -1 behind"]]})",
+     run_attn_evict},
     {"gdn.step",
      R"({"in":[["q","bf16","[B,NK,DK]"],["k","bf16","[B,NK,DK]"],["v","bf16","[B,NV,DV]"],["g","f32","[B,NV]"],["beta","bf16","[B,NV]"],["state_in","f32","[B,NV,DK,DV]"]],"out":[["o","bf16","[B,NV,DV]"],["state_out","f32","[B,NV,DK,DV]"]]})",
      run_gdn_step},

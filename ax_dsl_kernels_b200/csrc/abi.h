@@ -119,6 +119,11 @@ int run_attn_paged_decode(Call&);
 int run_attn_kv_write(Call&);
 int run_attn_lse_merge(Call&);
 int run_attn_paged_prefill(Call&);
+int run_attn_page_bounds(Call&);
+int run_attn_select_pages(Call&);
+int run_attn_sparse_decode(Call&);
+int run_attn_key_mass(Call&);
+int run_attn_evict(Call&);
 int run_gdn_step(Call&);
 int run_gdn_conv(Call&);
 int run_gdn_chunk_prefill(Call&);
