@@ -45,7 +45,7 @@ def lib():
             raise Q35Error(-1, f"{LIB_PATH} is missing: build it with `python -m ax_dsl_kernels_b200.build` "
                                "(there is no CPU or PyTorch fallback)")
         L = ctypes.CDLL(LIB_PATH)
-        L.q35_run.argtypes = [ctypes.c_char_p, ctypes.POINTER(_IO), ctypes.c_int, ctypes.c_void_p]
+        L.q35_run.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
         L.q35_run.restype = ctypes.c_int
         L.q35_workspace_bytes.argtypes = [ctypes.c_char_p, ctypes.POINTER(_IO), ctypes.c_int]
         L.q35_workspace_bytes.restype = ctypes.c_int64
@@ -101,44 +101,82 @@ def workspace_bytes(role, **tensors):
     return int(n)
 
 
-_ws_cache = {}
-_need_cache = {}
+_ws_cache = {}  # (device index, stream) -> (bytes, address, tensor)
 
 
-def _workspace(device, nbytes, stream=0):
-    """one growing scratch buffer per (device, stream), owned by the Python host (the library itself never allocates);
-    roles running concurrently on different streams must not share scratch"""
-    key = (device.type, device.index, stream)
-    buf = _ws_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _ws_cache[key] = buf
-    return buf
+def _workspace(dev, nbytes, stream):
+    """address of one growing scratch buffer per (device, stream), owned by the Python host (the library itself never
+    allocates); roles running concurrently on different streams must not share scratch"""
+    got = _ws_cache.get((dev, stream))
+    if got is None or got[0] < nbytes:
+        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", dev))
+        got = _ws_cache[dev, stream] = (buf.numel(), buf.data_ptr(), buf)
+    return got[1]
+
+
+class _Plan:
+    """What a call signature (role, names, dtypes, shapes) always binds: the IO table with everything but the pointers,
+    and the scratch the role needs.  `workspace`, when the role needs it and the caller brings none, is the last entry."""
+
+    def __init__(self, role, tensors):
+        self.role = role.encode()
+        self.need = workspace_bytes(role, **tensors) if "workspace" not in tensors else 0
+        if self.need:
+            tensors = dict(tensors, workspace=torch.empty(self.need, dtype=torch.uint8, device="meta"))
+        arr, self.names = _table(tensors)  # the table points at these names
+        self.n = len(tensors)
+        self.bytes = bytes(arr)
+        self.words = ctypes.c_uint64 * (len(self.bytes) // 8)
+
+
+_IO_WORDS, _PTR_WORD = ctypes.sizeof(_IO) // 8, _IO.ptr.offset // 8
+_plans = {}
+# the handle of a device's current stream without the Stream object around it (1.2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def run(role, stream=None, **tensors):
-    """q35_run(role, ...) with the given tensors bound by name; a `workspace` is added when the role needs one."""
+    """q35_run(role, ...) with the given tensors bound by name; a `workspace` is added when the role needs one.
+
+    The IO table of a signature is built (and checked) once and copied per call.  While a CUDA graph is being captured
+    the workspace comes from the graph's own memory: a graph must not hold the address of a buffer that a later, larger
+    call replaces, nor share one with another graph that may be replayed beside it."""
     L = lib()
-    dev = None
-    for t in tensors.values():
-        if not t.is_cuda:
+    ts = tensors.values()
+    devices = {t.get_device() for t in ts}
+    if len(devices) != 1 or -1 in devices:
+        if not devices or -1 in devices:
             raise ValueError("all tensors must live on the GPU (the library has no CPU path)")
-        dev = t.device
-    if "workspace" not in tensors:
-        # the scratch size depends on shapes and dtypes only: ask the library once per signature
-        sig = (role, tuple((n, t.dtype, tuple(t.shape)) for n, t in tensors.items()))
-        need = _need_cache.get(sig)
-        if need is None:
-            need = _need_cache[sig] = workspace_bytes(role, **tensors)
-        if stream is None:
-            stream = torch.cuda.current_stream(dev).cuda_stream
-        if need:
-            tensors = dict(tensors, workspace=_workspace(dev, need, stream))
-    arr, _keep = _table(tensors)
+        raise ValueError(f"the tensors are on different GPUs: {sorted(devices)}")
+    dev, = devices
+    sig = (role, tuple(tensors), tuple([t.dtype for t in ts]), tuple([t.shape for t in ts]))
+    if False in [t.is_contiguous() for t in ts]:
+        _table(tensors)  # names the tensor in its error
+    plan = _plans.get(sig)
+    if plan is None:
+        if len(_plans) >= 4096:  # shapes of a long-running server: page tables grow by the page
+            _plans.clear()
+        plan = _plans[sig] = _Plan(role, tensors)
+    ptrs = [t.data_ptr() for t in ts]
     if stream is None:
-        stream = torch.cuda.current_stream(dev).cuda_stream
-    with torch.cuda.device(dev):
-        _check(L.q35_run(role.encode(), arr, len(tensors), ctypes.c_void_p(stream)))
+        stream = _raw_stream(dev)
+    if plan.need:
+        if torch.cuda.is_current_stream_capturing():
+            own = torch.empty(plan.need, dtype=torch.uint8, device=torch.device("cuda", dev))
+            ptrs.append(own.data_ptr())
+        else:
+            ptrs.append(_workspace(dev, plan.need, stream))
+    table = plan.words.from_buffer_copy(plan.bytes)
+    i = _PTR_WORD
+    for p in ptrs:
+        table[i] = p
+        i += _IO_WORDS
+    if dev == torch.cuda.current_device():
+        _check(L.q35_run(plan.role, table, plan.n, stream))
+    else:
+        with torch.cuda.device(dev):
+            _check(L.q35_run(plan.role, table, plan.n, stream))
 
 
 def io_table(role):

@@ -493,6 +493,30 @@ def test_captured_and_replayed_and_on_another_stream():
     assert q35.device_status() == 0
 
 
+def test_a_captured_graph_keeps_its_own_scratch():
+    """a call that needs more scratch, made after the capture on the stream of the capture, replaces the eager buffer; the
+    graph's addresses stay valid and nobody else's"""
+    import ax_dsl_kernels_b200 as q35
+    cache, table, _, g = make([700, 900], 64, 2, 128, "bf16", 20)
+    gt, gc = gpu(table), gpu(cache)
+    q, gm = gpu(q_rows(2, 16, 128, g, 2.0)), torch.zeros((cache.shape[0], 64, 2), device="cuda")
+    want = q35.paged_attention_sparse(q, gc, *gt, key_mass=gm)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    out, gm2 = torch.empty_like(want), torch.zeros_like(gm)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        q35.paged_attention_sparse(q, gc, *gt, out=out, key_mass=gm2)
+    assert (q.get_device(), stream.cuda_stream) not in q35._lib._ws_cache
+    with torch.cuda.stream(stream):
+        for n in (1, 40):  # the second needs 40 times the first's
+            big = [torch.randn((64 * n, 4), device="cuda").sort().values for _ in range(2)]
+            ids, rw = torch.randint(0, 32, (64 * n, 4), dtype=torch.int32, device="cuda"), big[0].contiguous()
+            q35.moe_permute(ids, rw, 32, 16)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(gm, gm2)
+
+
 # ---------------------------------------------------------------------------------------------------- bad tables
 def test_bad_tables_are_recorded_and_touch_nothing():
     """page ids outside the cache, ranges outside the table, lists of pages that are not ascending"""
