@@ -43,8 +43,9 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
   const int last = a.keep ? min(max(a.keep[1], 0), K) : 0;
   const int first = a.keep ? min(max(a.keep[0], 0), K - last) : 0;
   const int m = n - first - last, rank = K - first - last;
+  bool bad = false;
   auto key = [&](int i) -> uint32_t {  // of position first + i
-    const int pos = first + i, page = max(0, page_at(a.t, sp.first + pos / a.t.P));
+    const int pos = first + i, page = page_or_first(a.t, sp.first + pos / a.t.P, bad);
     return order_key(a.key_mass[(size_t(page) * a.t.P + pos % a.t.P) * a.HKV + h]);
   };
   uint32_t border = 0;
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
     seen += total_eq;
     __syncthreads();
   }
+  if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
 }
 
 constexpr int EM_THREADS = 512;

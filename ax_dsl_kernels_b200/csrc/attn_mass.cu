@@ -59,18 +59,20 @@ struct KTile {
   float sc[LD];
 
   __device__ __forceinline__ void load(const MassArgs& a, const SeqPages& sp, int kvh, int k0) {
+    bool bad = false;
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int i = threadIdx.x + 256 * j, key = i / CPR, ch = i % CPR, pos = k0 + key;
       v[j] = make_uint4(0u, 0u, 0u, 0u);  // rows behind the end: zeros (their scores are masked)
       sc[j] = 0.f;
       if (pos < sp.ctx) {
-        const int page = max(0, page_at(a.t, sp.first + pos / a.t.P));
+        const int page = page_or_first(a.t, sp.first + pos / a.t.P, bad);
         const size_t row = (size_t(page) * 2 * a.t.P + pos % a.t.P) * a.HKV + kvh;
         v[j] = *reinterpret_cast<const uint4*>(a.cache + (row * CPR + ch) * 16);
         if constexpr (KVF == 2) sc[j] = __bfloat162float(a.row_scale[row]);
       }
     }
+    if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
   }
   __device__ __forceinline__ void store(uint8_t* tile) const {
 #pragma unroll

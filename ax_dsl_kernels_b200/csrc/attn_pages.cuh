@@ -14,7 +14,18 @@ struct PageTable {
   const int* last_page_len;  // [B]
   int B, P, num_pages, n_indices;
   int* status;
+  uint32_t p_mul; int p_shift;   // position / P as a high product and a shift
+  __device__ __forceinline__ int page_of(int pos) const {
+    return int((__umulhi(p_mul, uint32_t(pos)) + uint32_t(pos)) >> p_shift);
+  }
 };
+
+// 2^x by the special-function unit, 2 ulp; results below 2^-126 are 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // The pages of sequence b: indices[first .. first + n), n counting only pages that hold a row, ctx rows in all.
 // A range outside the table or a last page longer than P is recorded and the sequence counts as empty.
@@ -40,6 +51,15 @@ __device__ __forceinline__ int page_at(const PageTable& t, int e) {
   if (unsigned(id) < unsigned(t.num_pages)) return id;
   atomicOr(t.status, DS_BAD_PAGE);
   return -1;
+}
+
+// The same without the record: page 0 for an id that is none, which `bad` remembers.  A record on the spot would wait for
+// the id before the next instruction; callers that have several lookups on their way report once, behind them.
+__device__ __forceinline__ int page_or_first(const PageTable& t, int e, bool& bad) {
+  const int id = t.indices[e];
+  const bool no = unsigned(id) >= unsigned(t.num_pages);
+  bad |= no;
+  return no ? 0 : id;
 }
 
 // a float as an unsigned integer of the same order; NaN ranks with -inf, and -0 with 0
@@ -94,6 +114,11 @@ inline int get_page_table(Call& c, const char* role, int64_t B, int64_t P, int64
               (long long)P);
   t->indptr = indptr.as<int>(); t->indices = indices.as<int>(); t->last_page_len = last.as<int>();
   t->B = int(B); t->P = int(P); t->num_pages = int(num_pages); t->n_indices = int(indices.numel());
+  // n / P for n < 2^31: with 2^(l - 1) < P <= 2^l and m = floor(2^32 (2^l - P) / P) + 1, (umulhi(m, n) + n) >> l is exact
+  int l = 0;
+  while ((int64_t(1) << l) < P) ++l;
+  t->p_mul = uint32_t((uint64_t(1) << 32) * ((uint64_t(1) << l) - uint64_t(P)) / uint64_t(P) + 1);
+  t->p_shift = l;
   if (!c.dry) {
     t->status = device_status_ptr();
     Q35_REQUIRE(t->status != nullptr, Q35_ERR_CUDA, "%s: no device status word", role);

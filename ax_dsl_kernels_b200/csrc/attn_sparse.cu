@@ -7,7 +7,7 @@
 // Bound: HBM, K and V of the chosen rows once.  A cluster of C CTAs serves one (sequence, KV head): its chosen rows,
 // laid end to end, are cut into C contiguous ranges, every CTA runs one pass with a running maximum and sum over its
 // range, and the C partial results are merged through distributed shared memory -- one launch, no partials in HBM, no
-// counters.  Inside a CTA each warp owns groups of 16 rows and its own cp.async ring (16-byte chunks, XOR-swizzled
+// counters.  Inside a CTA each warp takes steps of 32 rows through its own cp.async ring (16-byte chunks, XOR-swizzled
 // rows), with no block barrier in the loop.  Scores are computed transposed (S^T = K Q^T, mma.m16n8k16) so that the up
 // to 8 query heads of a KV head are the n = 8 side and O^T takes D / 4 registers a lane.
 //
@@ -23,7 +23,8 @@ namespace q35 {
 namespace cg = cooperative_groups;
 
 constexpr int SP_G = 8;          // query heads per KV head handled by one mma column block
-constexpr int SP_KEYS = 16;      // rows per warp and step
+constexpr int SP_SUB = 16;       // rows of one MMA tile; a page holds whole tiles
+constexpr int SP_KEYS = 32;      // rows per warp and step
 constexpr float SP_LOG2E = 1.4426950408889634f;
 
 struct SparseArgs {
@@ -43,73 +44,42 @@ struct SparseArgs {
   int HQ, HKV, G, S;
 };
 
-// KVF: 0 bf16, 1 E4M3, 2 int8 rows with scales.  The one-byte formats arrive in half the time, so their dependent chain
-// (load fragments, convert, MMA, softmax, MMA) needs two warps per scheduler to hide; bf16 needs one.
+// KVF: 0 bf16, 1 E4M3, 2 int8 rows with scales.
+// A warp's step is 32 rows: K, then V, each a slot of its ring of three, so that 64 rows' worth of bytes are on their way
+// while one slot is in use.  32 rows (two MMA tiles) share one round of shuffles, exponentials' latency and rescaling;
+// 16-row steps took 5-25 % longer.  Four warps: 192 KB of ring and one CTA per SM with 512-byte rows, two or more with
+// narrower ones; eight warps per CTA were slower wherever lengths differ.
 template <int D, int KVF>
 struct SparseCfg {
   static constexpr bool BYTE = KVF != 0;
-  static constexpr int WARPS = BYTE ? 8 : 4;
-  static constexpr int STAGES = 3;
+  static constexpr int WARPS = 4;
+  static constexpr int SLOTS = 3;                       // half steps (32 rows of K or of V) per warp
   static constexpr int ROWB = D * (BYTE ? 1 : 2);
   static constexpr int CPR = ROWB / 16;                 // 16-byte chunks per row
   static constexpr int SWZ = (CPR < 8 ? CPR : 8) - 1;   // rows narrower than 128 bytes permute fewer chunks
-  static constexpr int KV_BYTES = SP_KEYS * ROWB;
-  static constexpr int STAGE_BYTES = 2 * KV_BYTES;
-  static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
+  static constexpr int SLOT_BYTES = SP_KEYS * ROWB;
+  static constexpr int RING = WARPS * SLOTS * SLOT_BYTES;
   static constexpr int PART = WARPS * SP_G * D * 4;     // the warps' output partials reuse the ring
   static constexpr int SMEM = RING > PART ? RING : PART;
-  static constexpr int LD = SP_KEYS * CPR / 32;         // chunks of K (and of V) per lane and step
+  static constexpr int LD = SP_KEYS * CPR / 32;         // chunks per lane and half step
 };
 
 template <int D, int KVF>
 __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decode_kernel(const SparseArgs a) {
   using C = SparseCfg<D, KVF>;
-  constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS, STAGES = C::STAGES;
+  constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_part[SP_G * D];                        // this CTA's merged output, read by the cluster
   __shared__ float s_ml[2 * SP_G];                          // its maxima and sums, read by the cluster
   __shared__ float s_wml[WARPS][2 * SP_G];
   __shared__ float s_fac[16][SP_G], s_fin[2 * SP_G], s_new[SP_G];
-  __shared__ int s_cut;
   pdl_wait();
   pdl_launch();
   cg::cluster_group cluster = cg::this_cluster();
   const int NC = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int row = blockIdx.x / NC, b = row / a.HKV, kvh = row % a.HKV;
-  const SeqPages sp = seq_pages(a.t, b);
-  const int P = a.t.P;
-
-  // the chosen pages: ascending positions in the sequence's page list; the list ends at the first entry that is not
-  const int* pages = a.pages ? a.pages + size_t(row) * a.S : nullptr;
-  int n_sel = sp.n, n_keys = sp.ctx;
-  if (pages) {
-    if (tid == 0) s_cut = a.S;
-    __syncthreads();
-    for (int i = tid; i < a.S; i += THREADS) {
-      const int p = pages[i], before = i ? pages[i - 1] : -1;
-      if (p < 0 || p >= sp.n || p <= before) {
-        if (p < -1 || (p >= 0 && before >= 0) || p >= sp.n) atomicOr(a.t.status, DS_BAD_PAGE);
-        atomicMin(&s_cut, i);
-      }
-    }
-    __syncthreads();
-    n_sel = s_cut;
-    n_keys = n_sel * P;
-    if (n_sel > 0 && pages[n_sel - 1] == sp.n - 1) n_keys += sp.ctx - sp.n * P;  // the last page may be part full
-  }
-  auto phys = [&](int slot) -> int { return page_at(a.t, sp.first + (pages ? pages[slot] : slot)); };
-
-  // groups of 16 rows: this CTA's contiguous range, dealt to its warps in turn
-  const int groups = (n_keys + SP_KEYS - 1) / SP_KEYS, per = (groups + NC - 1) / NC;
-  const int g_begin = min(groups, rank * per), g_end = min(groups, g_begin + per);
   const float scale_log2 = (a.sm_scale ? a.sm_scale[0] : rsqrtf(float(D))) * SP_LOG2E;
-  const size_t row_stride = size_t(a.HKV) * C::ROWB;  // bytes between consecutive rows of a page plane
-  // scores of this (sequence, KV head): behind S * P rows of every row of the grid, or behind the table entries before
-  float* scores = a.scores;
-  if (scores)
-    scores += (pages ? size_t(row) * a.S : size_t(a.HKV) * sp.first + size_t(kvh) * sp.n) * size_t(P) * SP_G;
-
   // query fragments (B operand, heads on the n side).  bf16 / int8 cache: bf16 (int8: in the k order the byte-wise
   // fragments come out in).  E4M3: f16, after scaling each head by the power of two that brings its largest element to
   // [2^14, 2^15): exact but for elements 2^-28 times smaller, which lose bits below 2^-39 of the largest.
@@ -155,49 +125,94 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
     }
   }
 
-  const uint32_t sbase = smem_u32(smem) + warp * (STAGES * C::STAGE_BYTES);
-  const int first_group = g_begin + warp;
-  // physical page of a group (16 rows lie in one page: P is a multiple of 16), looked up ahead of its use
-  auto group_page = [&](int g) -> int {
-    if (g >= g_end) return 0;
-    const int p = phys(g * SP_KEYS / P);
-    return p < 0 ? 0 : p;
+  const SeqPages sp = seq_pages(a.t, b);
+  const int P = a.t.P;
+
+  // the chosen pages: ascending positions in the sequence's page list; the list ends at the first entry that is not.
+  // Every warp reads the whole list for itself: no barrier before the first row can be asked for.
+  const int* pages = a.pages ? a.pages + size_t(row) * a.S : nullptr;
+  int n_sel = sp.n, n_keys = sp.ctx;
+  if (pages) {
+    int before = -1;
+    n_sel = a.S;
+    for (int i0 = 0; i0 < a.S; i0 += 32) {
+      const int p = i0 + lane < a.S ? pages[i0 + lane] : -1;
+      const int left = __shfl_up_sync(0xffffffffu, p, 1);
+      const int prev = lane ? left : before;
+      const unsigned end = __ballot_sync(0xffffffffu, p < 0 || p >= sp.n || p <= prev);
+      const int cut = end ? __ffs(end) - 1 : 32;
+      before = __shfl_sync(0xffffffffu, p, cut ? cut - 1 : 0);
+      if (!end) continue;
+      if (lane == cut && p != -1) atomicOr(a.t.status, DS_BAD_PAGE);  // not the end of the list, but no page
+      n_sel = min(a.S, i0 + cut);
+      if (!cut && i0) before = pages[i0 - 1];
+      break;
+    }
+    n_keys = n_sel * P;
+    if (n_sel > 0 && before == sp.n - 1) n_keys += sp.ctx - sp.n * P;  // the last page may be part full
+  }
+
+  // steps of 32 rows: this CTA's contiguous range, dealt to its warps in turn
+  const int steps = (n_keys + SP_KEYS - 1) / SP_KEYS, per = (steps + NC - 1) / NC;
+  const int s_begin = min(steps, rank * per), s_end = min(steps, s_begin + per);
+  const size_t row_stride = size_t(a.HKV) * C::ROWB;  // bytes between consecutive rows of a page plane
+  // scores of this (sequence, KV head): behind S * P rows of every row of the grid, or behind the table entries before
+  float* scores = a.scores;
+  if (scores)
+    scores += (pages ? size_t(row) * a.S : size_t(a.HKV) * sp.first + size_t(kvh) * sp.n) * size_t(P) * SP_G;
+
+  // Where the warp's next 32 tiles of 16 rows lie, one lane each: tile u of the warp is half u & 1 of its step u / 2.
+  // Looked up 32 at a time, a round ahead, so that no step waits for the page table or divides by P.
+  const int first_step = s_begin + warp, my_steps = first_step < s_end ? (s_end - first_step + WARPS - 1) / WARPS : 0;
+  auto tile_row = [&](int u) { return (first_step + (u >> 1) * WARPS) * SP_KEYS + (u & 1) * SP_SUB; };
+  auto entry_of = [&](int u) -> int {  // position in the page list of the sequence, -1 behind the end
+    const int k = tile_row(u);
+    return u < 2 * my_steps && k < n_keys ? (pages ? pages[a.t.page_of(k)] : a.t.page_of(k)) : -1;
   };
-  auto issue = [&](int g, int page) {
-    if (g < g_end) {
-      const int ro = g * SP_KEYS % P, valid = min(SP_KEYS, n_keys - g * SP_KEYS);
-      const uint8_t* kb = a.cache + (size_t(page) * 2 * P + ro) * row_stride + size_t(kvh) * C::ROWB;
-      const uint8_t* vb = kb + size_t(P) * row_stride;
-      const uint32_t st = sbase + ((g - first_group) / WARPS % STAGES) * C::STAGE_BYTES;
+  int page_cur, row_cur, entry_next;  // page and row in it of tile (round * 32 + lane); entry of the next round's
+  auto look_up = [&](int u0, int entry) {
+    const int id = entry >= 0 ? page_at(a.t, sp.first + entry) : 0;
+    page_cur = id < 0 ? 0 : id;
+    const int k = tile_row(u0 + lane);
+    row_cur = entry >= 0 ? k - a.t.page_of(k) * P : 0;
+  };
+  look_up(0, entry_of(lane));
+  entry_next = entry_of(32 + lane);
+
+  const uint32_t sbase = smem_u32(smem) + warp * (C::SLOTS * C::SLOT_BYTES);
+  // 32 rows of K (kv 0) or V (kv 1) of the warp's step i into slot (2 i + kv) % 3
+  auto issue = [&](int i, int kv, int slot) {
+    if (i < my_steps) {
+      const int left = n_keys - (first_step + i * WARPS) * SP_KEYS;
+      const uint32_t st = sbase + slot * C::SLOT_BYTES;
 #pragma unroll
-      for (int j = 0; j < C::LD; ++j) {
-        const int ci = lane + 32 * j, key = ci / C::CPR, ch = ci % C::CPR;
-        const uint32_t at = st + key * C::ROWB + ((ch ^ (key & C::SWZ)) << 4);
-        if (key < valid) {
-          cp_async_16(at, kb + size_t(key) * row_stride + ch * 16);
-          cp_async_16(at + C::KV_BYTES, vb + size_t(key) * row_stride + ch * 16);
-        } else {  // rows behind the end are never read: zeros keep 0 * V a zero
-          asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u));
-          asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + C::KV_BYTES), "r"(0u));
+      for (int half = 0; half < 2; ++half) {
+        const int src = (2 * i + half) & 31;
+        const int page = __shfl_sync(0xffffffffu, page_cur, src), ro = __shfl_sync(0xffffffffu, row_cur, src);
+        const uint8_t* base = a.cache + ((size_t(page) * 2 + kv) * P + ro) * row_stride + size_t(kvh) * C::ROWB;
+#pragma unroll
+        for (int j = 0; j < C::LD / 2; ++j) {
+          const int ci = lane + 32 * j, key = ci / C::CPR, ch = ci % C::CPR, at_key = half * SP_SUB + key;
+          const uint32_t at = st + at_key * C::ROWB + ((ch ^ (key & C::SWZ)) << 4);
+          if (at_key < left)
+            cp_async_16(at, base + size_t(key) * row_stride + ch * 16);
+          else if (kv == 1)  // rows behind the end are never read: zeros keep 0 * V a zero
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0u));
         }
       }
     }
     cp_async_commit();
   };
-  // int8: the row scales this lane's fragments need -- K rows r and r + 8, V rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9 -- two
-  // groups ahead in registers; 0 for rows behind the end
-  auto load_scales = [&](int g, int page) -> uint3 {
-    uint3 v = make_uint3(0u, 0u, 0u);
+  // int8: the row scales of a step, lane l holding K (low half) and V of row l; 0 behind the end
+  auto load_scales = [&](int i) -> uint32_t {
+    uint32_t v = 0u;
     if constexpr (KVF == 2) {
-      if (g < g_end) {
-        const int ro = g * SP_KEYS % P, valid = n_keys - g * SP_KEYS;
-        const unsigned short* ks = reinterpret_cast<const unsigned short*>(a.row_scale) +
-                                   (size_t(page) * 2 * P + ro) * a.HKV + kvh;
-        const unsigned short* vs = ks + size_t(P) * a.HKV;
-        auto at = [&](const unsigned short* s, int i) -> uint32_t { return i < valid ? s[size_t(i) * a.HKV] : 0u; };
-        v.x = at(ks, r) | at(ks, r + 8) << 16;
-        v.y = at(vs, 2 * c) | at(vs, 2 * c + 1) << 16;
-        v.z = at(vs, 2 * c + 8) | at(vs, 2 * c + 9) << 16;
+      const int src = (2 * i + (lane >> 4)) & 31;
+      const int page = __shfl_sync(0xffffffffu, page_cur, src), ro = __shfl_sync(0xffffffffu, row_cur, src);
+      if (i < my_steps && (first_step + i * WARPS) * SP_KEYS + lane < n_keys) {
+        const unsigned short* sp16 = reinterpret_cast<const unsigned short*>(a.row_scale) +
+                                     (size_t(page) * 2 * P + ro + (lane & 15)) * a.HKV + kvh;
+        v = uint32_t(sp16[0]) | uint32_t(sp16[size_t(P) * a.HKV]) << 16;
       }
     }
     return v;
@@ -208,91 +223,138 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
   for (int mt = 0; mt < D / 16; ++mt) oacc[mt][0] = oacc[mt][1] = oacc[mt][2] = oacc[mt][3] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 
-  uint3 rs_cur, rs_n1, rs_n2;
-  {
-    const int p0 = group_page(first_group), p1 = group_page(first_group + WARPS);
-    issue(first_group, p0);
-    issue(first_group + WARPS, p1);
-    rs_cur = load_scales(first_group, p0);
-    rs_n1 = load_scales(first_group + WARPS, p1);
-  }
-  static_assert(STAGES == 3, "two groups in flight ahead of the one in use");
-  int page_next = group_page(first_group + 2 * WARPS);
-
-  for (int g = first_group; g < g_end; g += WARPS) {
-    issue(g + 2 * WARPS, page_next);
-    rs_n2 = load_scales(g + 2 * WARPS, page_next);
-    page_next = group_page(g + 3 * WARPS);
-    cp_async_wait<STAGES - 1>();
+  // half steps in flight: while K of step i is in use, V of step i and K of step i + 1 are on their way, then V of both
+  issue(0, 0, 0);
+  issue(0, 1, 1);
+  uint32_t rs_next = load_scales(0);
+  int slot = 0;  // of the half step in use
+  for (int i = 0; i < my_steps; ++i) {
+    const uint32_t rs = rs_next;
+    if (((i + 1) & 15) == 0) {  // the next step is the first of another round of 32 tiles
+      look_up(2 * (i + 1), entry_next);
+      entry_next = entry_of(2 * (i + 1) + 32 + lane);
+    }
+    issue(i + 1, 0, slot == 0 ? 2 : slot - 1);
+    rs_next = load_scales(i + 1);
+    cp_async_wait<2>();
     __syncwarp();
-    const int valid = min(SP_KEYS, n_keys - g * SP_KEYS);
-    const uint32_t st = sbase + ((g - first_group) / WARPS % STAGES) * C::STAGE_BYTES;
-    float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const int step = first_step + i * WARPS, left = n_keys - step * SP_KEYS;
+    uint32_t st = sbase + slot * C::SLOT_BYTES;
+    float sacc[2][2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sacc[h][0][u] = sacc[h][1][u] = 0.f;
     {
       const int key = (lane & 7) + (((lane >> 3) & 1) << 3);
       const uint32_t rowa = st + key * C::ROWB;
       if constexpr (!C::BYTE) {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const int ch = 2 * ks + (lane >> 4);
-          uint32_t a0, a1, a2, a3;
-          ldmatrix_x4(rowa + ((ch ^ (key & C::SWZ)) << 4), a0, a1, a2, a3);
-          mma_bf16_16816(sacc[ks & 1], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
+        for (int k0 = 0; k0 < D / 16; k0 += 2) {
+          uint32_t f[2][2][4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int ch = 2 * (k0 + k) + (lane >> 4);
+              ldmatrix_x4(rowa + h * SP_SUB * C::ROWB + ((ch ^ (key & C::SWZ)) << 4), f[k][h][0], f[k][h][1], f[k][h][2],
+                          f[k][h][3]);
+            }
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              mma_bf16_16816(sacc[h][k], f[k][h][0], f[k][h][1], f[k][h][2], f[k][h][3], qf[k0 + k][0], qf[k0 + k][1]);
         }
       } else {
+        float ks[2][2];  // int8: scales of the rows r and r + 8 of both tiles
+        if constexpr (KVF == 2) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) ks[h][u] = bf16lo(__shfl_sync(0xffffffffu, rs, h * 16 + u * 8 + r));
+        }
 #pragma unroll
         for (int kp = 0; kp < D / 32; ++kp) {  // 32 channels: two mma over bytes taken as b16 pairs
           const int ch = 2 * kp + (lane >> 4);
-          uint32_t r0, r1, r2, r3;
-          ldmatrix_x4(rowa + ((ch ^ (key & C::SWZ)) << 4), r0, r1, r2, r3);
-          if constexpr (KVF == 2) {
-            const float s0 = bf16lo(rs_cur.x), s1 = bf16hi(rs_cur.x);
-            r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
-            mma_bf16_16816(sacc[0], cvt_s8x2_bf16x2<0, 1>(r0, s0, s0), cvt_s8x2_bf16x2<0, 1>(r1, s1, s1),
-                           cvt_s8x2_bf16x2<2, 3>(r0, s0, s0), cvt_s8x2_bf16x2<2, 3>(r1, s1, s1), qf[2 * kp][0],
-                           qf[2 * kp][1]);
-            mma_bf16_16816(sacc[1], cvt_s8x2_bf16x2<0, 1>(r2, s0, s0), cvt_s8x2_bf16x2<0, 1>(r3, s1, s1),
-                           cvt_s8x2_bf16x2<2, 3>(r2, s0, s0), cvt_s8x2_bf16x2<2, 3>(r3, s1, s1), qf[2 * kp + 1][0],
-                           qf[2 * kp + 1][1]);
-          } else {
-            mma_f16_16816(sacc[0], cvt_kv<0, 1>(r0), cvt_kv<0, 1>(r1), cvt_kv<2, 3>(r0), cvt_kv<2, 3>(r1),
-                          qf[2 * kp][0], qf[2 * kp][1]);
-            mma_f16_16816(sacc[1], cvt_kv<0, 1>(r2), cvt_kv<0, 1>(r3), cvt_kv<2, 3>(r2), cvt_kv<2, 3>(r3),
-                          qf[2 * kp + 1][0], qf[2 * kp + 1][1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r0, r1, r2, r3;
+            ldmatrix_x4(rowa + h * SP_SUB * C::ROWB + ((ch ^ (key & C::SWZ)) << 4), r0, r1, r2, r3);
+            if constexpr (KVF == 2) {
+              const float s0 = ks[h][0], s1 = ks[h][1];
+              r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
+              mma_bf16_16816(sacc[h][0], cvt_s8x2_bf16x2<0, 1>(r0, s0, s0), cvt_s8x2_bf16x2<0, 1>(r1, s1, s1),
+                             cvt_s8x2_bf16x2<2, 3>(r0, s0, s0), cvt_s8x2_bf16x2<2, 3>(r1, s1, s1), qf[2 * kp][0],
+                             qf[2 * kp][1]);
+              mma_bf16_16816(sacc[h][1], cvt_s8x2_bf16x2<0, 1>(r2, s0, s0), cvt_s8x2_bf16x2<0, 1>(r3, s1, s1),
+                             cvt_s8x2_bf16x2<2, 3>(r2, s0, s0), cvt_s8x2_bf16x2<2, 3>(r3, s1, s1), qf[2 * kp + 1][0],
+                             qf[2 * kp + 1][1]);
+            } else {
+              mma_f16_16816(sacc[h][0], cvt_kv<0, 1>(r0), cvt_kv<0, 1>(r1), cvt_kv<2, 3>(r0), cvt_kv<2, 3>(r1),
+                            qf[2 * kp][0], qf[2 * kp][1]);
+              mma_f16_16816(sacc[h][1], cvt_kv<0, 1>(r2), cvt_kv<0, 1>(r3), cvt_kv<2, 3>(r2), cvt_kv<2, 3>(r3),
+                            qf[2 * kp + 1][0], qf[2 * kp + 1][1]);
+            }
           }
         }
       }
     }
-    float sc[4];  // rows r, r, r + 8, r + 8; heads 2 c, 2 c + 1
+    __syncwarp();  // K's slot is free
+    issue(i + 1, 1, slot);
+    slot = slot == 2 ? 0 : slot + 1;
+    st = sbase + slot * C::SLOT_BYTES;
+    float sc[2][4];  // rows r, r, r + 8, r + 8 of both tiles; heads 2 c, 2 c + 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      sc[i] = r + ((i >> 1) << 3) < valid ? (sacc[0][i] + sacc[1][i]) * col_scale[i & 1] : -INFINITY;
-    if (scores) {
-      float* at = scores + (size_t(g) * SP_KEYS + r) * SP_G + 2 * c;
-      if (r < valid) *reinterpret_cast<float2*>(at) = make_float2(sc[0], sc[1]);
-      if (r + 8 < valid) *reinterpret_cast<float2*>(at + 8 * SP_G) = make_float2(sc[2], sc[3]);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        sc[h][u] = h * SP_SUB + r + ((u >> 1) << 3) < left ? (sacc[h][0][u] + sacc[h][1][u]) * col_scale[u & 1] : -INFINITY;
+      if (scores) {
+        float* at = scores + (size_t(step) * SP_KEYS + h * SP_SUB + r) * SP_G + 2 * c;
+        if (h * SP_SUB + r < left) *reinterpret_cast<float2*>(at) = make_float2(sc[h][0], sc[h][1]);
+        if (h * SP_SUB + r + 8 < left) *reinterpret_cast<float2*>(at + 8 * SP_G) = make_float2(sc[h][2], sc[h][3]);
+      }
     }
-    float mt2[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
+    float top[2] = {fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2])),
+                    fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3]))};
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
-      mt2[0] = fmaxf(mt2[0], __shfl_xor_sync(0xffffffffu, mt2[0], o));
-      mt2[1] = fmaxf(mt2[1], __shfl_xor_sync(0xffffffffu, mt2[1], o));
+      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
     }
-    // E4M3: weights 2^8 times larger, up to 256, so that the f16 pair that carries them resolves 2^-32 of the maximum
+    // E4M3: weights 2^8 times larger, up to 256, so that f16 resolves 2^-32 of the largest
     constexpr float LIFT = KVF == 1 ? 8.f : 0.f;
     float alpha[2], ref[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float mn = fmaxf(m_run[h], mt2[h]);
+      const float mn = fmaxf(m_run[h], top[h]);
       const float base = mn == -INFINITY ? 0.f : mn;  // no row with a weight yet
-      alpha[h] = exp2f(m_run[h] - base);
+      alpha[h] = ex2(m_run[h] - base);
       m_run[h] = mn;
       ref[h] = base - LIFT;
     }
-    const float p0 = exp2f(sc[0] - ref[0]), p1 = exp2f(sc[1] - ref[1]);
-    const float p2 = exp2f(sc[2] - ref[0]), p3 = exp2f(sc[3] - ref[1]);
-    l_run[0] = l_run[0] * alpha[0] + p0 + p2;
-    l_run[1] = l_run[1] * alpha[1] + p1 + p3;
+    // bf16 / int8: P enters the P V product as two bf16 terms (p = hi + lo); one alone, 2^-8, would cost as much as the
+    // output's own rounding.  E4M3: one f16 term, 2^-11, an eighth of it (a second one: 58 -> 60 us for 32 sequences of up to 4161 rows).
+    uint32_t pb[2][2], pl[2][2];  // pl: unused for E4M3
+    l_run[0] *= alpha[0];
+    l_run[1] *= alpha[1];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {  // rows r, then r + 8
+        const float p0 = ex2(sc[h][2 * u] - ref[0]), p1 = ex2(sc[h][2 * u + 1] - ref[1]);
+        l_run[0] += p0;
+        l_run[1] += p1;
+        if constexpr (KVF == 1) {
+          pb[h][u] = movmatrix_trans(pack_f16(p0, p1));
+        } else {
+          const float h0 = round_bf16(p0), h1 = round_bf16(p1);
+          pb[h][u] = movmatrix_trans(pack_bf16(h0, h1));
+          pl[h][u] = movmatrix_trans(pack_bf16(p0 - h0, p1 - h1));
+        }
+      }
+    }
     if (alpha[0] != 1.f || alpha[1] != 1.f) {
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt) {
@@ -300,71 +362,73 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
         oacc[mt][2] *= alpha[0]; oacc[mt][3] *= alpha[1];
       }
     }
-    // P enters the P V product as two 16-bit terms (p = hi + lo): one alone would cost as much as the output's rounding
+    cp_async_wait<2>();
+    __syncwarp();
     if constexpr (!C::BYTE) {
-      const float h0 = round_bf16(p0), h1 = round_bf16(p1), h2 = round_bf16(p2), h3 = round_bf16(p3);
-      const uint32_t pb0 = movmatrix_trans(pack_bf16(h0, h1)), pb1 = movmatrix_trans(pack_bf16(h2, h3));
-      const uint32_t pl0 = movmatrix_trans(pack_bf16(p0 - h0, p1 - h1));
-      const uint32_t pl1 = movmatrix_trans(pack_bf16(p2 - h2, p3 - h3));
       const int key = (lane & 7) + ((lane >> 4) << 3);
-      const uint32_t rowa = st + C::KV_BYTES + key * C::ROWB;
+      const uint32_t rowa = st + key * C::ROWB;
+      constexpr int MB = 4;  // output tiles whose fragments are fetched together: dependent products lie MB apart
 #pragma unroll
-      for (int mt = 0; mt < D / 16; ++mt) {
-        const int ch = 2 * mt + ((lane >> 3) & 1);
-        uint32_t a0, a1, a2, a3;
-        ldmatrix_x4_trans(rowa + ((ch ^ (key & C::SWZ)) << 4), a0, a1, a2, a3);
-        mma_bf16_16816(oacc[mt], a0, a1, a2, a3, pb0, pb1);
-        mma_bf16_16816(oacc[mt], a0, a1, a2, a3, pl0, pl1);
+      for (int m0 = 0; m0 < D / 16; m0 += MB) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t f[MB][4];
+#pragma unroll
+          for (int m = 0; m < MB; ++m) {
+            const int ch = 2 * (m0 + m) + ((lane >> 3) & 1);
+            ldmatrix_x4_trans(rowa + h * SP_SUB * C::ROWB + ((ch ^ (key & C::SWZ)) << 4), f[m][0], f[m][1], f[m][2], f[m][3]);
+          }
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+            mma_bf16_16816(oacc[m0 + m], f[m][0], f[m][1], f[m][2], f[m][3], pb[h][0], pb[h][1]);
+#pragma unroll
+          for (int m = 0; m < MB; ++m)
+            mma_bf16_16816(oacc[m0 + m], f[m][0], f[m][1], f[m][2], f[m][3], pl[h][0], pl[h][1]);
+        }
       }
     } else {
       // transposed b16 loads keep byte pairs (d, d + 1) together: bytes (0, 2) / (1, 3) are the row pairs of channels
       // 2 r / 2 r + 1, so mma row r holds channel 16 mt + 2 r and mma row r + 8 channel 16 mt + 2 r + 1
-      uint32_t pb0, pb1, pl0, pl1;
+      float vs[2][4];  // int8: scales of the rows 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of both tiles
       if constexpr (KVF == 2) {
-        const float h0 = round_bf16(p0), h1 = round_bf16(p1), h2 = round_bf16(p2), h3 = round_bf16(p3);
-        pb0 = movmatrix_trans(pack_bf16(h0, h1));
-        pb1 = movmatrix_trans(pack_bf16(h2, h3));
-        pl0 = movmatrix_trans(pack_bf16(p0 - h0, p1 - h1));
-        pl1 = movmatrix_trans(pack_bf16(p2 - h2, p3 - h3));
-      } else {
-        auto hi = [](float p) { return __half2float(__float2half_rn(p)); };
-        const float h0 = hi(p0), h1 = hi(p1), h2 = hi(p2), h3 = hi(p3);
-        pb0 = movmatrix_trans(pack_f16(h0, h1));
-        pb1 = movmatrix_trans(pack_f16(h2, h3));
-        pl0 = movmatrix_trans(pack_f16(p0 - h0, p1 - h1));
-        pl1 = movmatrix_trans(pack_f16(p2 - h2, p3 - h3));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            vs[h][u] = bf16hi(__shfl_sync(0xffffffffu, rs, h * 16 + 2 * c + (u & 1) + ((u >> 1) << 3)));
       }
       const int key = lane & 15;
-      const uint32_t rowa = st + C::KV_BYTES + key * C::ROWB;
+      const uint32_t rowa = st + key * C::ROWB;
 #pragma unroll
       for (int mp = 0; mp < D / 32; ++mp) {
         const int ch = 2 * mp + (lane >> 4);
-        uint32_t r0, r1, r2, r3;  // (rows 0-7, chunk 2 mp) (rows 8-15, 2 mp) (rows 0-7, 2 mp + 1) (rows 8-15, 2 mp + 1)
-        ldmatrix_x4_trans(rowa + ((ch ^ (key & C::SWZ)) << 4), r0, r1, r2, r3);
-        if constexpr (KVF == 2) {
-          const float va = bf16lo(rs_cur.y), vb = bf16hi(rs_cur.y), vc = bf16lo(rs_cur.z), vd = bf16hi(rs_cur.z);
-          r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
-          const uint32_t a0 = cvt_s8x2_bf16x2<0, 2>(r0, va, vb), a1 = cvt_s8x2_bf16x2<1, 3>(r0, va, vb);
-          const uint32_t a2 = cvt_s8x2_bf16x2<0, 2>(r1, vc, vd), a3 = cvt_s8x2_bf16x2<1, 3>(r1, vc, vd);
-          mma_bf16_16816(oacc[2 * mp], a0, a1, a2, a3, pb0, pb1);
-          mma_bf16_16816(oacc[2 * mp], a0, a1, a2, a3, pl0, pl1);
-          const uint32_t b0 = cvt_s8x2_bf16x2<0, 2>(r2, va, vb), b1 = cvt_s8x2_bf16x2<1, 3>(r2, va, vb);
-          const uint32_t b2 = cvt_s8x2_bf16x2<0, 2>(r3, vc, vd), b3 = cvt_s8x2_bf16x2<1, 3>(r3, vc, vd);
-          mma_bf16_16816(oacc[2 * mp + 1], b0, b1, b2, b3, pb0, pb1);
-          mma_bf16_16816(oacc[2 * mp + 1], b0, b1, b2, b3, pl0, pl1);
-        } else {
-          const uint32_t a0 = cvt_kv<0, 2>(r0), a1 = cvt_kv<1, 3>(r0), a2 = cvt_kv<0, 2>(r1), a3 = cvt_kv<1, 3>(r1);
-          mma_f16_16816(oacc[2 * mp], a0, a1, a2, a3, pb0, pb1);
-          mma_f16_16816(oacc[2 * mp], a0, a1, a2, a3, pl0, pl1);
-          const uint32_t b0 = cvt_kv<0, 2>(r2), b1 = cvt_kv<1, 3>(r2), b2 = cvt_kv<0, 2>(r3), b3 = cvt_kv<1, 3>(r3);
-          mma_f16_16816(oacc[2 * mp + 1], b0, b1, b2, b3, pb0, pb1);
-          mma_f16_16816(oacc[2 * mp + 1], b0, b1, b2, b3, pl0, pl1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r0, r1, r2, r3;  // (rows 0-7, chunk 2 mp) (rows 8-15, 2 mp) (rows 0-7, 2 mp + 1) (rows 8-15, 2 mp + 1)
+          ldmatrix_x4_trans(rowa + h * SP_SUB * C::ROWB + ((ch ^ (key & C::SWZ)) << 4), r0, r1, r2, r3);
+          uint32_t x[8];
+          if constexpr (KVF == 2) {
+            const float va = vs[h][0], vb = vs[h][1], vc = vs[h][2], vd = vs[h][3];
+            r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
+            x[0] = cvt_s8x2_bf16x2<0, 2>(r0, va, vb); x[1] = cvt_s8x2_bf16x2<1, 3>(r0, va, vb);
+            x[2] = cvt_s8x2_bf16x2<0, 2>(r1, vc, vd); x[3] = cvt_s8x2_bf16x2<1, 3>(r1, vc, vd);
+            x[4] = cvt_s8x2_bf16x2<0, 2>(r2, va, vb); x[5] = cvt_s8x2_bf16x2<1, 3>(r2, va, vb);
+            x[6] = cvt_s8x2_bf16x2<0, 2>(r3, vc, vd); x[7] = cvt_s8x2_bf16x2<1, 3>(r3, vc, vd);
+            mma_bf16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[h][0], pb[h][1]);
+            mma_bf16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[h][0], pb[h][1]);
+            mma_bf16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pl[h][0], pl[h][1]);
+            mma_bf16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pl[h][0], pl[h][1]);
+          } else {
+            x[0] = cvt_kv<0, 2>(r0); x[1] = cvt_kv<1, 3>(r0); x[2] = cvt_kv<0, 2>(r1); x[3] = cvt_kv<1, 3>(r1);
+            x[4] = cvt_kv<0, 2>(r2); x[5] = cvt_kv<1, 3>(r2); x[6] = cvt_kv<0, 2>(r3); x[7] = cvt_kv<1, 3>(r3);
+            mma_f16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[h][0], pb[h][1]);
+            mma_f16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[h][0], pb[h][1]);
+          }
         }
       }
     }
-    __syncwarp();
-    rs_cur = rs_n1;
-    rs_n1 = rs_n2;
+    __syncwarp();  // V's slot is free
+    slot = slot == 2 ? 0 : slot + 1;
   }
   cp_async_wait<0>();
   __syncthreads();  // the ring is free: the warps' partials go there
@@ -408,12 +472,12 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_wml[w][tid]);
     const float base = m == -INFINITY ? 0.f : m;
     for (int w = 0; w < WARPS; ++w) {
-      const float f = exp2f(s_wml[w][tid] - base);
+      const float f = ex2(s_wml[w][tid] - base);
       s_fac[w][tid] = f;
       l += s_wml[w][SP_G + tid] * f;
     }
     if (has_new) {
-      const float f = exp2f(s_new[tid] - base) * LIFTED;
+      const float f = ex2(s_new[tid] - base) * LIFTED;
       s_fac[15][tid] = f;
       l += f;
     }
@@ -443,7 +507,7 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
     for (int k = 0; k < NC; ++k) m = fmaxf(m, s_cm[k][tid]);
     const float base = m == -INFINITY ? 0.f : m;
     for (int k = 0; k < NC; ++k) {
-      const float f = exp2f(s_cm[k][tid] - base);
+      const float f = ex2(s_cm[k][tid] - base);
       s_fac[k][tid] = f;
       l += s_cl[k][tid] * f;
     }
@@ -466,21 +530,40 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
         pack_bf16(o0 * inv, o1 * inv);
   }
   if (a.key_mass) {
-    // the lifted weights' sums are 2^LIFT times larger: so is what a score stands for
-    for (int k = g_begin * SP_KEYS + tid; k < min(n_keys, g_end * SP_KEYS); k += THREADS) {
-      const float4 s0 = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G);
-      const float4 s1 = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G + 4);
-      const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-      float w = 0.f;
+    // Four rows of every thread on their way together, no branch between them: rows behind the end read the last row's
+    // scores and add nothing.  (One warp per scheduler: what counts here is the number of instructions per row.)
+    constexpr int U = 4;
+    const int k_begin = s_begin * SP_KEYS, k_end = min(n_keys, s_end * SP_KEYS);
+    float top[SP_G], inv[SP_G];
 #pragma unroll
-      for (int g = 0; g < SP_G; ++g)
-        if (g < a.G) w += exp2f(s[g] - s_fin[g]) * s_fin[SP_G + g];
-      const int page = phys(k / P);
-      if (page >= 0) atomicAdd(a.key_mass + (size_t(page) * P + k % P) * a.HKV + kvh, w * LIFTED);
+    for (int g = 0; g < SP_G; ++g) {
+      top[g] = s_fin[g];
+      inv[g] = g < a.G ? s_fin[SP_G + g] * LIFTED : 0.f;
+    }
+    for (int k0 = k_begin + tid; k0 < k_end; k0 += U * THREADS) {
+      float4 lo[U], hi[U];
+      int page[U], off[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = min(k0 + u * THREADS, k_end - 1), e = a.t.page_of(k);
+        lo[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G);
+        hi[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G + 4);
+        page[u] = a.t.indices[sp.first + (pages ? pages[e] : e)];  // no page: recorded by the step that read the row
+        off[u] = k - e * P;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float s[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+        float w = 0.f;
+#pragma unroll
+        for (int g = 0; g < SP_G; ++g) w += inv[g] == 0.f ? 0.f : ex2(s[g] - top[g]) * inv[g];
+        if (k0 + u * THREADS < k_end && unsigned(page[u]) < unsigned(a.t.num_pages))
+          atomicAdd(a.key_mass + (size_t(page[u]) * P + off[u]) * a.HKV + kvh, w);
+      }
     }
     if (has_new && tid == 0) {
       float w = 0.f;
-      for (int g = 0; g < a.G; ++g) w += exp2f(s_new[g] - s_fin[g]) * s_fin[SP_G + g];
+      for (int g = 0; g < a.G; ++g) w += ex2(s_new[g] - s_fin[g]) * s_fin[SP_G + g];
       const int page = a.new_at[2 * b], off = a.new_at[2 * b + 1];
       if (unsigned(page) < unsigned(a.t.num_pages) && unsigned(off) < unsigned(P))
         a.key_mass[(size_t(page) * P + off) * a.HKV + kvh] = w * LIFTED;
@@ -491,25 +574,49 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decod
   cluster.sync();  // no CTA leaves while another still reads its shared memory
 }
 
+// CTAs per (sequence, KV head).  `slots` CTAs are resident at a time.
+// Chosen pages: all rows of the grid have about the same length, the most CTAs that still run at once (64 sequences x
+// 2 heads x 4096 rows on 148 slots: 1 CTA 92 us, 2: 95, 4: 112).  All pages: lengths differ, so at least one CTA per
+// slot, and more to even them out (32 x 4 ragged E4M3 rows on 296 slots: 2 CTAs 65 us, 4: 60, 8: 76).
+// Never more than one step per warp; 16 (beyond the portable 8) for a few long rows.
+static int sparse_cluster(int64_t rows, int64_t steps, int slots, bool chosen) {
+  int c = 1;
+  while (c < 8 && (chosen ? rows * c * 2 <= slots : rows * c < slots)) c *= 2;
+  if (c == 8 && rows * 16 <= slots && steps >= 16 * 32) c = 16;
+  while (c > 1 && c / 2 * 4 >= steps) c /= 2;
+  return c;
+}
+
 template <int D, int KVF>
-static int launch_sparse(const SparseArgs& a, int cluster, cudaStream_t stream) {
+static int launch_sparse(const SparseArgs& a, cudaStream_t stream) {
   using C = SparseCfg<D, KVF>;
   const void* f = reinterpret_cast<const void*>(sparse_decode_kernel<D, KVF>);
   // the 48 KB that need no opt-in hold the static arrays too: head_dim 64 is above them with exactly 48 KB of ring
   Q35_TRY(ensure_dynamic_smem(f, C::SMEM > 49 * 1024 ? C::SMEM : 49 * 1024));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(a.t.B) * a.HKV * cluster);
-  cfg.blockDim = dim3(32 * C::WARPS);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(cluster); attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr; cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sparse_decode_kernel<D, KVF>, a);
-  Q35_REQUIRE(e == cudaSuccess, Q35_ERR_CUDA, "attn.sparse_decode: %s", cudaGetErrorString(e));
+  const int resident = 200 * 1024 / C::SMEM < 1 ? 1 : 200 * 1024 / C::SMEM;
+  const int64_t rows = int64_t(a.t.B) * a.HKV;
+  const int64_t keys = int64_t(a.t.P) * (a.pages ? a.S : (a.t.n_indices + a.t.B - 1) / a.t.B);
+  const int cluster = sparse_cluster(rows, (keys + SP_KEYS - 1) / SP_KEYS, (resident < 2 ? 1 : 2) * sm_count(), a.pages != nullptr);
+  cudaError_t e = cudaSuccess;
+  if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(rows * cluster));
+    cfg.blockDim = dim3(32 * C::WARPS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster); attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, sparse_decode_kernel<D, KVF>, a);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the caller's next CUDA call
+    return fail(Q35_ERR_CUDA, "attn.sparse_decode: %s", cudaGetErrorString(e));
+  }
   Q35_CUDA_LAUNCH_CHECK("attn.sparse_decode");
   return 0;
 }
@@ -533,7 +640,7 @@ int run_attn_sparse_decode(Call& c) {
   Q35_REQUIRE(HQ / HKV <= SP_G, Q35_ERR_UNSUPPORTED, "%s: at most 8 query heads per KV head (got %lld)", role,
               (long long)(HQ / HKV));
   Q35_REQUIRE(D == 64 || D == 128 || D == 256, Q35_ERR_UNSUPPORTED, "%s: head_dim must be 64/128/256", role);
-  Q35_REQUIRE(P % SP_KEYS == 0, Q35_ERR_UNSUPPORTED, "%s: page size must be a multiple of 16", role);
+  Q35_REQUIRE(P % SP_SUB == 0, Q35_ERR_UNSUPPORTED, "%s: page size must be a multiple of 16", role);
   Q35_REQUIRE(out.numel() == B * HQ * D, Q35_ERR_SHAPE, "%s: out [B, HQ, D]", role);
   Q35_REQUIRE(!pages.present || (pages.nd == 3 && pages.s[0] == B && pages.s[1] == HKV && pages.s[2] >= 1), Q35_ERR_SHAPE,
               "%s: pages [B, HKV, S]", role);
@@ -564,10 +671,9 @@ int run_attn_sparse_decode(Call& c) {
   a.key_mass = mass.present ? mass.as<float>() : nullptr;
   a.scores = mass.present ? ws.as<float>() : nullptr;
   a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(HQ / HKV); a.S = int(S);
-  const int cluster = 8;
-#define Q35_SPARSE(DD)                                                          \
-  (kv.fmt == 0 ? launch_sparse<DD, 0>(a, cluster, c.stream)                     \
-               : kv.fmt == 1 ? launch_sparse<DD, 1>(a, cluster, c.stream) : launch_sparse<DD, 2>(a, cluster, c.stream))
+#define Q35_SPARSE(DD)                                                 \
+  (kv.fmt == 0 ? launch_sparse<DD, 0>(a, c.stream) : kv.fmt == 1 ? launch_sparse<DD, 1>(a, c.stream) \
+                                                                 : launch_sparse<DD, 2>(a, c.stream))
   if (D == 64) return Q35_SPARSE(64);
   if (D == 128) return Q35_SPARSE(128);
   return Q35_SPARSE(256);
