@@ -4,11 +4,15 @@
 // For a page with keys k_1 .. k_m let lo_d = min_i k_id and hi_d = max_i k_id.  Then q . k_i <= sum_d max(q_d lo_d,
 // q_d hi_d) for every key of the page, and the right side costs 1 / (P / 2) of the products with all P keys.  A KV head
 // is shared by G query heads, so a page's score is the maximum of the G bounds.
+#include <cooperative_groups.h>
 #include "abi.h"
 #include "attn_pages.cuh"
+#include "block_select.cuh"
 #include "kv_formats.cuh"
 
 namespace q35 {
+
+namespace cg = cooperative_groups;
 
 // ---------------------------------------------------------------------------------------------------------------
 // attn.page_bounds.  Bound: HBM (the K rows are read once, the bounds are 2 / P of them).  The K rows of a page are one
@@ -206,22 +210,35 @@ int run_attn_page_bounds(Call& c) {
 // The order of the scores decides, and two summation orders of the same bf16 products can disagree about two close
 // pages.  So the scores are found twice: sum_d max(q_d lo_d, q_d hi_d) = max(q, 0) . hi + min(q, 0) . lo is a product
 // of bf16 rows that the tensor cores do for all heads at once in fp32, with an error of at most n 2^-23 sum |terms| for
-// any order of n = 2 D terms; and the few pages within that error of the border (usually one to ten) are scored again
-// in fp64, where the sum of 512 products of 16 significant bits is as good as exact.
-// Bound: HBM for the bounds (each read once); at one sequence the launch and the chain of the selection.
+// any order of n = 2 D terms, and a third product, |q| . max(|lo|, |hi|), bounds that sum; the few pages within that
+// error of the border (most often one to three) are scored again in fp64, where the sum of 512 products of 16
+// significant bits is as good as exact.  (An infinite bound turns 0 * inf of the split form into a NaN and the error
+// into infinity: then every page is scored again, by the definition.)
+//
+// Bound: HBM for the bounds (each read once); at one sequence the chain of the selection.  One launch: a cluster of up
+// to 8 CTAs scores the pages of one (sequence, KV head) and leaves the scores in the shared memory of its first CTA,
+// which chooses (two kernels with the scores in HBM between them: 21.6 us instead of 10.0 for 256 pages, 31.8 instead of 18.0 for 32 rows of 2048).
 struct SelectArgs {
   const __nv_bfloat16* q;       // [B, HQ, D]
   const __nv_bfloat16* bounds;  // [pages, 2, HKV, D]
   PageTable t;                  // P unused
   const int* keep;              // optional [2]: first, last
   int* out;                     // [B, HKV, S]
-  int HQ, HKV, G, D, S, gx;
-  // workspace, [HKV * n_indices] each: entries of (b, kvh) start at HKV * indptr[b] + kvh * n
-  float2* score;                // score and its error bound
-  double* zscore;               // fp64 scores of the zone
-  int* zone;                    // pages of the zone
-  uint8_t* flag;                // 0 out, 1 in, 2 zone
+  int HQ, HKV, G, S;
+  int cap;                      // pages whose scores and flags fit the shared memory
+  // workspace, [HKV * n_indices] each, entries of (b, kvh) from HKV * indptr[b] + kvh * n on: where more is needed than
+  // fits the shared memory
+  float* score;
+  uint8_t* flag;                // 0 out, 1 in, 2 undecided
+  double* zscore;               // fp64 scores of the undecided pages
+  int* zone;                    // their positions
 };
+
+constexpr int SEL_THREADS = 512, SEL_WARPS = 16;
+constexpr int SEL_CAP = 16384;     // pages of a sequence that stay in shared memory
+constexpr int SEL_KEYS = 4;        // pages per thread and round of the output
+static_assert(SEL_KEYS * SEL_WARPS == 64, "the output's scan takes two counts a lane");
+constexpr int SEL_ZONE = 512;      // undecided pages that stay in shared memory
 
 // pages of sequence b that hold a row, without knowing P
 __device__ __forceinline__ int2 select_range(const SelectArgs& a, int b) {
@@ -232,10 +249,6 @@ __device__ __forceinline__ int2 select_range(const SelectArgs& a, int b) {
   }
   return make_int2(lo, hi - lo - (hi > lo && a.t.last_page_len[b] <= 0 ? 1 : 0));
 }
-__device__ __forceinline__ int select_page(const SelectArgs& a, int e) {
-  const int id = page_at(a.t, e);
-  return id < 0 ? 0 : id;
-}
 __device__ __forceinline__ uint32_t pos_pair(uint32_t x) {
   __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
   return *reinterpret_cast<uint32_t*>(&v);
@@ -244,102 +257,100 @@ __device__ __forceinline__ uint32_t neg_pair(uint32_t x) {
   __nv_bfloat162 v = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ float max_nan(float x, float y) { return x != x ? x : y != y ? y : fmaxf(x, y); }
-
-// One warp scores 16 pages: A = the pages' hi and lo rows, B = max(q, 0) and min(q, 0) of 8 heads.  Both operands take
-// their k index from 16-byte loads (lane c of a row's four holds channels 8 c .. 8 c + 7 of every 32), so the fragments
-// come straight from global memory and a row is read in full sectors.
-template <int D>
-__global__ void __launch_bounds__(128) select_score_kernel(const SelectArgs a) {
-  pdl_wait();
-  pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int row = blockIdx.x / a.gx, b = row / a.HKV, h = row % a.HKV;
-  const int2 rg = select_range(a, b);
-  const int n = rg.y;
-  const size_t base = size_t(a.HKV) * rg.x + size_t(h) * n;
-  for (int p0 = ((blockIdx.x % a.gx) * 4 + warp) * 16; p0 < n; p0 += a.gx * 64) {
-    const int i0 = min(p0 + r, n - 1), i1 = min(p0 + r + 8, n - 1);
-    const size_t plane = size_t(a.HKV) * D;
-    const __nv_bfloat16* lo0 = a.bounds + size_t(select_page(a, rg.x + i0)) * 2 * plane + size_t(h) * D + 8 * c;
-    const __nv_bfloat16* lo1 = a.bounds + size_t(select_page(a, rg.x + i1)) * 2 * plane + size_t(h) * D + 8 * c;
-    float best0 = -INFINITY, best1 = -INFINITY, q1max = 0.f, kmax0 = 0.f, kmax1 = 0.f;
-    for (int g0 = 0; g0 < a.G; g0 += 8) {
-      const bool hv = g0 + r < a.G;
-      const __nv_bfloat16* qp = a.q + (size_t(b) * a.HQ + size_t(h) * a.G + (hv ? g0 + r : 0)) * D + 8 * c;
-      float ap[4] = {0.f, 0.f, 0.f, 0.f}, an[4] = {0.f, 0.f, 0.f, 0.f};
-      float q1 = 0.f;
-      uint32_t km0 = 0u, km1 = 0u;
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint4 l0 = ldg_nc_16(lo0 + j * 32), l1 = ldg_nc_16(lo1 + j * 32);
-        const uint4 h0 = ldg_nc_16(lo0 + plane + j * 32), h1 = ldg_nc_16(lo1 + plane + j * 32);
-        uint4 qv = make_uint4(0u, 0u, 0u, 0u);
-        if (hv) qv = *reinterpret_cast<const uint4*>(qp + j * 32);
-        mma_bf16_16816(ap, h0.x, h1.x, h0.y, h1.y, pos_pair(qv.x), pos_pair(qv.y));
-        mma_bf16_16816(an, l0.x, l1.x, l0.y, l1.y, neg_pair(qv.x), neg_pair(qv.y));
-        mma_bf16_16816(ap, h0.z, h1.z, h0.w, h1.w, pos_pair(qv.z), pos_pair(qv.w));
-        mma_bf16_16816(an, l0.z, l1.z, l0.w, l1.w, neg_pair(qv.z), neg_pair(qv.w));
-        const uint32_t qw[4] = {qv.x, qv.y, qv.z, qv.w};
-        const uint32_t w0[8] = {l0.x, l0.y, l0.z, l0.w, h0.x, h0.y, h0.z, h0.w};
-        const uint32_t w1[8] = {l1.x, l1.y, l1.z, l1.w, h1.x, h1.y, h1.z, h1.w};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) q1 += fabsf(bf16lo(qw[u])) + fabsf(bf16hi(qw[u]));
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {  // largest magnitude of the rows' bounds: bf16 magnitudes order as integers
-          km0 = __vmaxu2(km0, w0[u] & 0x7fff7fffu);
-          km1 = __vmaxu2(km1, w1[u] & 0x7fff7fffu);
-        }
-      }
-      q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
-      q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
-      q1max = fmaxf(q1max, q1);  // of head r of this block of heads; over the heads below
-      kmax0 = fmaxf(kmax0, fmaxf(bf16lo(km0), bf16hi(km0)));
-      kmax1 = fmaxf(kmax1, fmaxf(bf16lo(km1), bf16hi(km1)));
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (g0 + 2 * c + u < a.G) {
-          best0 = max_nan(best0, ap[u] + an[u]);
-          best1 = max_nan(best1, ap[2 + u] + an[2 + u]);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      best0 = max_nan(best0, __shfl_xor_sync(0xffffffffu, best0, o));
-      best1 = max_nan(best1, __shfl_xor_sync(0xffffffffu, best1, o));
-      kmax0 = fmaxf(kmax0, __shfl_xor_sync(0xffffffffu, kmax0, o));
-      kmax1 = fmaxf(kmax1, __shfl_xor_sync(0xffffffffu, kmax1, o));
-    }
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) q1max = fmaxf(q1max, __shfl_xor_sync(0xffffffffu, q1max, o));
-    if (c == 0) {  // 2 D terms of at most |q|_1 kmax in all: an error of 2 D 2^-23 of that at most
-      const float rel = 2.f * D / 8388608.f;
-      if (p0 + r < n) a.score[base + p0 + r] = make_float2(best0, q1max * kmax0 * rel);
-      if (p0 + r + 8 < n) a.score[base + p0 + r + 8] = make_float2(best1, q1max * kmax1 * rel);
-    }
-  }
+// larger magnitudes of two pairs (a NaN gives way to a number)
+__device__ __forceinline__ uint32_t abs_max_pair(uint32_t x, uint32_t y) {
+  x &= 0x7fff7fffu;
+  y &= 0x7fff7fffu;
+  __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<__nv_bfloat162*>(&y));
+  return *reinterpret_cast<uint32_t*>(&v);
 }
-
+__device__ __forceinline__ float max_nan(float x, float y) { return x != x ? x : y != y ? y : fmaxf(x, y); }
 __device__ __forceinline__ unsigned long long order_key64(double x) {
   if (x != x) x = -INFINITY;
   const unsigned long long u = __double_as_longlong(x + 0.0);
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The r-th largest (r >= 1) of key(0 .. n - 1), digit by digit from the top: a histogram of the digits of the keys that
-// agree with the prefix so far, then the digit in which the rank falls.  above = how many keys are larger.
-template <typename K, typename F>
-__device__ K block_kth_largest(F key, int n, int r, int* hist, int* above) {
+// One warp scores the 16 pages from p0 on: A = the pages' hi and lo rows, B = max(q, 0) and min(q, 0) of 8 heads.  Both
+// operands take their k index from 16-byte loads (lane c of a row's four holds channels 8 c .. 8 c + 7 of every 32), so
+// the fragments come straight from global memory and a row is read in full sectors.  Returns the largest error bound.
+template <int D>
+__device__ __forceinline__ float score_pages(const SelectArgs& a, int b, int h, int first, int n, int p0, float* score) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const size_t plane = size_t(a.HKV) * D;
+  bool bad = false;
+  const int g0 = page_or_first(a.t, first + min(p0 + r, n - 1), bad);
+  const int g1 = page_or_first(a.t, first + min(p0 + r + 8, n - 1), bad);
+  const uint4* lo0 = reinterpret_cast<const uint4*>(a.bounds + size_t(g0) * 2 * plane + size_t(h) * D + 8 * c);
+  const uint4* lo1 = reinterpret_cast<const uint4*>(a.bounds + size_t(g1) * 2 * plane + size_t(h) * D + 8 * c);
+  const size_t up = plane / 8;  // from a minimum to its maximum, in 16-byte pieces
+  float best0 = -INFINITY, best1 = -INFINITY, err = 0.f;
+  for (int q0 = 0; q0 < a.G; q0 += 8) {
+    const bool hv = q0 + r < a.G;
+    const uint4* qp = reinterpret_cast<const uint4*>(a.q + (size_t(b) * a.HQ + size_t(h) * a.G + (hv ? q0 + r : 0)) * D + 8 * c);
+    float ap[4] = {0.f, 0.f, 0.f, 0.f}, an[4] = {0.f, 0.f, 0.f, 0.f}, as[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int NB = D / 32 < 4 ? D / 32 : 4;  // 32-channel pieces whose loads go out together
+#pragma unroll
+    for (int j0 = 0; j0 < D / 32; j0 += NB) {
+      uint4 l0[NB], l1[NB], h0[NB], h1[NB], qv[NB];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        l0[j] = __ldg(lo0 + (j0 + j) * 4);
+        l1[j] = __ldg(lo1 + (j0 + j) * 4);
+        h0[j] = __ldg(lo0 + up + (j0 + j) * 4);
+        h1[j] = __ldg(lo1 + up + (j0 + j) * 4);
+        qv[j] = hv ? __ldg(qp + (j0 + j) * 4) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        mma_bf16_16816(ap, h0[j].x, h1[j].x, h0[j].y, h1[j].y, pos_pair(qv[j].x), pos_pair(qv[j].y));
+        mma_bf16_16816(an, l0[j].x, l1[j].x, l0[j].y, l1[j].y, neg_pair(qv[j].x), neg_pair(qv[j].y));
+        mma_bf16_16816(as, abs_max_pair(h0[j].x, l0[j].x), abs_max_pair(h1[j].x, l1[j].x), abs_max_pair(h0[j].y, l0[j].y),
+                       abs_max_pair(h1[j].y, l1[j].y), qv[j].x & 0x7fff7fffu, qv[j].y & 0x7fff7fffu);
+        mma_bf16_16816(ap, h0[j].z, h1[j].z, h0[j].w, h1[j].w, pos_pair(qv[j].z), pos_pair(qv[j].w));
+        mma_bf16_16816(an, l0[j].z, l1[j].z, l0[j].w, l1[j].w, neg_pair(qv[j].z), neg_pair(qv[j].w));
+        mma_bf16_16816(as, abs_max_pair(h0[j].z, l0[j].z), abs_max_pair(h1[j].z, l1[j].z), abs_max_pair(h0[j].w, l0[j].w),
+                       abs_max_pair(h1[j].w, l1[j].w), qv[j].z & 0x7fff7fffu, qv[j].w & 0x7fff7fffu);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (q0 + 2 * c + u < a.G) {
+        best0 = max_nan(best0, ap[u] + an[u]);
+        best1 = max_nan(best1, ap[2 + u] + an[2 + u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) err = fmaxf(err, as[u]);  // a NaN here comes with a score that is NaN, and ranks last
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    best0 = max_nan(best0, __shfl_xor_sync(0xffffffffu, best0, o));
+    best1 = max_nan(best1, __shfl_xor_sync(0xffffffffu, best1, o));
+  }
+  if (c == 0) {
+    if (p0 + r < n) score[p0 + r] = best0;
+    if (p0 + r + 8 < n) score[p0 + r + 8] = best1;
+  }
+  if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
+  // 2 D terms, the three sums' own roundings, the final addition: (2 D + 8) 2^-23, and 1 + 2^-9 for `as` being rounded
+  return err * ((2 * D + 8) * (1.f + 1.f / 512) / 8388608.f);
+}
+
+// The r-th largest (r >= 1) of the 64-bit keys key(0 .. n - 1), digit by digit from the top: a histogram of the digits of
+// the keys that agree with the prefix so far, then the digit in which the rank falls.  above = how many keys are larger.
+template <typename F>
+__device__ unsigned long long block_kth64(F key, int n, int r, int* hist, int* above) {
   __shared__ int s_digit, s_rank;
+  using K = unsigned long long;
   K prefix = 0;
   int rank = r;
-  for (int shift = int(sizeof(K)) * 8 - 8; shift >= 0; shift -= 8) {
+  for (int shift = 56; shift >= 0; shift -= 8) {
     for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       const K k = key(i);
-      if (shift == int(sizeof(K)) * 8 - 8 || ((k ^ prefix) >> (shift + 8)) == 0) atomicAdd(&hist[int(k >> shift) & 255], 1);
+      if (shift == 56 || ((k ^ prefix) >> (shift + 8)) == 0) atomicAdd(&hist[int(k >> shift) & 255], 1);
     }
     __syncthreads();
     if (threadIdx.x < 32) {  // lane l sums the digits 255 - 8 l .. 248 - 8 l, then the warp scans from the top
@@ -374,151 +385,251 @@ __device__ K block_kth_largest(F key, int n, int r, int* hist, int* above) {
   return prefix;
 }
 
-constexpr int SEL_THREADS = 1024;
-
-// one CTA per (sequence, KV head): the choice
 template <int D>
-__global__ void __launch_bounds__(SEL_THREADS) select_choose_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(SEL_THREADS, 1) select_kernel(const SelectArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_err[8 * SEL_WARPS];  // one entry per warp of the cluster
+  __shared__ KthScratch<SEL_THREADS> s_kth;
+  __shared__ int s_hist[256];
+  __shared__ int s_red[2][SEL_WARPS], s_count[SEL_KEYS][SEL_WARPS], s_total;
+  __shared__ int s_zone[SEL_ZONE];
+  __shared__ double s_zscore[SEL_ZONE];
+  __shared__ int s_nz;
   pdl_wait();
   pdl_launch();
-  __shared__ int s_hist[256];
-  __shared__ int s_scan[32];
-  __shared__ float s_max[32];
-  __shared__ int s_zone;
+  cg::cluster_group cluster = cg::this_cluster();
+  auto started = cluster.barrier_arrive();  // its shared memory is written from outside once the first CTA runs
+  const int NC = int(cluster.num_blocks()), crank = int(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x, b = row / a.HKV, h = row % a.HKV;
+  const int row = blockIdx.x / NC, b = row / a.HKV, h = row % a.HKV;
   const int2 rg = select_range(a, b);
   const int n = rg.y, S = a.S;
+  const size_t base = size_t(a.HKV) * rg.x + size_t(h) * n;
+  float* s_score = reinterpret_cast<float*>(smem);
+  const bool fits = n <= a.cap;
+  cluster.barrier_wait(std::move(started));
+  if (n > S) {
+    float* score = fits ? cluster.map_shared_rank(s_score, 0) : a.score + base;
+    float err = 0.f;
+    for (int p0 = (warp * NC + crank) * 16; p0 < n; p0 += NC * SEL_WARPS * 16)
+      err = fmaxf(err, score_pages<D>(a, b, h, rg.x, n, p0, score));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
+    if (lane == 0) cluster.map_shared_rank(s_err, 0)[crank * SEL_WARPS + warp] = err;
+  }
+  if (!fits) __threadfence();
+  cluster.sync();
+  if (crank) return;  // only the first CTA's memory is read from here on
   int* out = a.out + size_t(row) * S;
   if (n <= S) {
     for (int i = tid; i < S; i += SEL_THREADS) out[i] = i < n ? i : -1;
     return;
   }
-  const size_t base = size_t(a.HKV) * rg.x + size_t(h) * n;
-  const float2* score = a.score + base;
-  uint8_t* flag = a.flag + base;
-  int last = a.keep ? min(max(a.keep[1], 0), S) : 0;
+  const float* score = fits ? s_score : a.score + base;
+  uint8_t* flag = fits ? smem + size_t(a.cap) * 4 : a.flag + base;
+  const int last = a.keep ? min(max(a.keep[1], 0), S) : 0;
   const int first = a.keep ? min(max(a.keep[0], 0), S - last) : 0;
   const int m = n - first - last, rank = S - first - last;  // rank of the m free pages; rank < m because S < n
-  // largest error bound of a free page (inf and NaN: every page is scored again)
-  float e = 0.f;
-  for (int i = tid; i < m; i += SEL_THREADS) e = max_nan(e, score[first + i].y);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) e = max_nan(e, __shfl_xor_sync(0xffffffffu, e, o));
-  if (lane == 0) s_max[warp] = e;
-  if (tid == 0) s_zone = 0;
-  __syncthreads();
-  e = s_max[0];
-  for (int w = 1; w < 32; ++w) e = max_nan(e, s_max[w]);
-  const bool all = !(e < INFINITY);
-  int in = 0;  // pages certainly chosen
   if (rank > 0) {
-    int above;
-    const uint32_t kth = block_kth_largest<uint32_t>([&](int i) { return order_key(score[first + i].x); }, m, rank, s_hist,
-                                                     &above);
+    float e = 0.f;
+    for (int w = 0; w < NC * SEL_WARPS; ++w) e = fmaxf(e, s_err[w]);
+    const bool all = !(e < INFINITY);  // sums that overflow fp32: every page is scored again
+    uint32_t kth;
+    if (m <= 4 * SEL_THREADS) {
+      uint32_t k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) k[j] = tid + j * SEL_THREADS < m ? order_key(score[first + tid + j * SEL_THREADS]) : 0u;
+      kth = block_kth<SEL_THREADS, true>(
+          [&](auto f) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (tid + j * SEL_THREADS < m) f(k[j]);
+          },
+          rank, s_kth);
+    } else {
+      kth = block_kth<SEL_THREADS, true>(
+          [&](auto f) {
+            for (int i = tid; i < m; i += SEL_THREADS) f(order_key(score[first + i]));
+          },
+          rank, s_kth);
+    }
     // the rank-th score as a float again; a true score differs from its fp32 one by e at most, so does the border
-    const float tau = __uint_as_float(kth & 0x80000000u ? kth & 0x7fffffffu : ~kth);
+    const float tau = key_value(kth);
     const float top = tau + 2.f * e, low = tau - 2.f * e;
+    int in = 0, near = 0;
     for (int i = tid; i < m; i += SEL_THREADS) {
-      const float s = score[first + i].x;
-      int f;
-      if (all || !(s > top || s < low)) {
-        f = 2;
-        a.zone[base + atomicAdd(&s_zone, 1)] = first + i;
-      } else {
-        f = s > top;
-        in += f;
-      }
+      const float s = score[first + i];
+      const int f = all || !(s > top || s < low) ? 2 : s > top;
+      in += f == 1;
+      near += f == 2;
       flag[first + i] = uint8_t(f);
     }
-    for (int o = 16; o; o >>= 1) in += __shfl_xor_sync(0xffffffffu, in, o);
-    if (lane == 0) s_scan[warp] = in;
+    in = __reduce_add_sync(0xffffffffu, in);
+    near = __reduce_add_sync(0xffffffffu, near);
+    if (lane == 0) { s_red[0][warp] = in; s_red[1][warp] = near; }
     __syncthreads();
     in = 0;
-    for (int w = 0; w < 32; ++w) in += s_scan[w];
-    const int z = s_zone, need = rank - in;  // need <= z: the zone holds the border
+    int z = 0;  // undecided pages
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; ++w) { in += s_red[0][w]; z += s_red[1][w]; }
+    const int need = rank - in;  // 1 <= need <= z: the zone holds the border
     const size_t plane = size_t(a.HKV) * D;
-    for (int j = warp; j < z; j += 32) {
-      const int i = a.zone[base + j];
-      const __nv_bfloat16* lo = a.bounds + size_t(select_page(a, rg.x + i)) * 2 * plane + size_t(h) * D;
-      double best = -INFINITY;
-      bool nan = false;
-      for (int g = 0; g < a.G; ++g) {
-        const __nv_bfloat16* qp = a.q + (size_t(b) * a.HQ + size_t(h) * a.G + g) * D;
-        double sum = 0.;
-        for (int d = lane; d < D; d += 32) {
-          const float q = __bfloat162float(qp[d]);
-          const float qpos = q != q ? q : fmaxf(q, 0.f), qneg = q != q ? q : fminf(q, 0.f);
-          sum += double(qpos) * double(__bfloat162float(lo[plane + d])) + double(qneg) * double(__bfloat162float(lo[d]));
-        }
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        nan |= sum != sum;
-        best = fmax(best, sum);
-      }
-      if (lane == 0) a.zscore[base + i] = nan ? -INFINITY : best;
-    }
-    __syncthreads();
-    const int* zone = a.zone + base;
-    const double* zs = a.zscore + base;
-    if (z <= 2048) {  // each page of the zone counts the pages that go before it
-      for (int j = tid; j < z; j += SEL_THREADS) {
+    if (z == need) {  // nothing undecided
+      for (int i = tid; i < m; i += SEL_THREADS) flag[first + i] = flag[first + i] != 0;
+    } else {
+      int* zone = z <= SEL_ZONE ? s_zone : a.zone + base;
+      double* zs = z <= SEL_ZONE ? s_zscore : a.zscore + base;
+      if (tid == 0) s_nz = 0;
+      __syncthreads();
+      for (int i = tid; i < m; i += SEL_THREADS)
+        if (flag[first + i] == 2) zone[atomicAdd(&s_nz, 1)] = first + i;
+      __syncthreads();
+      for (int j = warp; j < z; j += SEL_WARPS) {
         const int i = zone[j];
-        const double s = zs[i];
-        int before = 0;
-        for (int k = 0; k < z; ++k) {
-          const int i2 = zone[k];
-          const double s2 = zs[i2];
-          before += s2 > s || (s2 == s && i2 < i);
+        bool bad = false;
+        const __nv_bfloat16* lo = a.bounds + size_t(page_or_first(a.t, rg.x + i, bad)) * 2 * plane + size_t(h) * D;
+        // every lane its D / 32 channels of the page, eight heads' partial sums at a time; folding halves of the warp
+        // leaves lane l the sum of head (l >> 2) & 7
+        // A channel's term is q * hi for q > 0 and q * lo for q < 0; for q = 0 it is 0, or NaN beside an infinite bound.
+        constexpr int CH = D / 32;
+        double l[CH], u[CH], z0[CH];
+#pragma unroll
+        for (int i = 0; i < CH; i += 2) {
+          const uint32_t l2 = *reinterpret_cast<const uint32_t*>(lo + lane * CH + i);
+          const uint32_t u2 = *reinterpret_cast<const uint32_t*>(lo + plane + lane * CH + i);
+          l[i] = bf16lo(l2); l[i + 1] = bf16hi(l2); u[i] = bf16lo(u2); u[i + 1] = bf16hi(u2);
+          z0[i] = bf16lo(l2) * 0.f + bf16lo(u2) * 0.f;
+          z0[i + 1] = bf16hi(l2) * 0.f + bf16hi(u2) * 0.f;
         }
-        flag[i] = before < need;
-      }
-    } else {  // pages that hardly differ: the border by digits, equal ones by index below
-      int above64;
-      const unsigned long long k64 = block_kth_largest<unsigned long long>(
-          [&](int j) { return order_key64(zs[zone[j]]); }, z, need, s_hist, &above64);
-      for (int j = tid; j < z; j += SEL_THREADS) {
-        const int i = zone[j];
-        const unsigned long long k = order_key64(zs[i]);
-        flag[i] = k > k64 ? 1 : k < k64 ? 0 : 2;
+        double best = -INFINITY;
+        for (int q0 = 0; q0 < a.G; q0 += 8) {
+          double sum[8];
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const __nv_bfloat16* qp = a.q + (size_t(b) * a.HQ + size_t(h) * a.G + min(q0 + g, a.G - 1)) * D + lane * CH;
+            sum[g] = 0.;
+#pragma unroll
+            for (int i = 0; i < CH; i += 2) {
+              const uint32_t q2 = *reinterpret_cast<const uint32_t*>(qp + i);
+              const float qa = bf16lo(q2), qb = bf16hi(q2);
+              sum[g] += double(qa) * (qa > 0.f ? u[i] : qa < 0.f ? l[i] : z0[i]);
+              sum[g] += double(qb) * (qb > 0.f ? u[i + 1] : qb < 0.f ? l[i + 1] : z0[i + 1]);
+            }
+          }
+#pragma unroll
+          for (int half = 4; half; half >>= 1)
+#pragma unroll
+            for (int g = 0; g < half; ++g) {
+              const bool up = lane & (half * 4);
+              const double other = __shfl_xor_sync(0xffffffffu, up ? sum[g] : sum[g + half], half * 4);
+              sum[g] = (up ? sum[g + half] : sum[g]) + other;
+            }
+          sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
+          sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+          best = best != best || sum[0] != sum[0] ? NAN : fmax(best, sum[0]);
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          const double other = __shfl_xor_sync(0xffffffffu, best, o);
+          best = best != best || other != other ? NAN : fmax(best, other);
+        }
+        if (lane == 0) zs[j] = best != best ? -INFINITY : best;
       }
       __syncthreads();
-      // of the pages equal to the border (flag 2) the first need - above64 in order
-      int left = need - above64;
-      for (int i0 = 0; i0 < m; i0 += SEL_THREADS) {
-        const int i = first + i0 + tid;
-        const bool eq = i0 + tid < m && flag[i] == 2;
-        const unsigned ball = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) s_scan[warp] = __popc(ball);
-        __syncthreads();
-        int before = __popc(ball & ((1u << lane) - 1)), total = 0;
-        for (int w = 0; w < 32; ++w) {
-          if (w < warp) before += s_scan[w];
-          total += s_scan[w];
+      if (z <= SEL_ZONE) {  // each page of the zone counts the pages that go before it
+        for (int j = tid; j < z; j += SEL_THREADS) {
+          const int i = zone[j];
+          const double s = zs[j];
+          int before = 0;
+          for (int k = 0; k < z; ++k) before += zs[k] > s || (zs[k] == s && zone[k] < i);
+          flag[i] = before < need;
         }
-        if (eq) flag[i] = before < left;
-        left = max(0, left - total);
+      } else {  // pages that hardly differ: the border by digits, equal ones by position
+        int above;
+        const unsigned long long k64 =
+            block_kth64([&](int j) { return order_key64(zs[j]); }, z, need, s_hist, &above);
+        for (int j = tid; j < z; j += SEL_THREADS) {
+          const unsigned long long k = order_key64(zs[j]);
+          flag[zone[j]] = k > k64 ? 1 : k < k64 ? 0 : 2;
+        }
         __syncthreads();
+        int left = need - above;  // of the pages equal to the border (flag 2) the first `left` in order
+        for (int i0 = 0; i0 < m; i0 += SEL_THREADS) {
+          const int i = first + i0 + tid;
+          const bool eq = i0 + tid < m && flag[i] == 2;
+          const unsigned ball = __ballot_sync(0xffffffffu, eq);
+          if (lane == 0) s_red[0][warp] = __popc(ball);
+          __syncthreads();
+          int before = __popc(ball & ((1u << lane) - 1)), total = 0;
+          for (int w = 0; w < SEL_WARPS; ++w) {
+            if (w < warp) before += s_red[0][w];
+            total += s_red[0][w];
+          }
+          if (eq) flag[i] = before < left;
+          left = max(0, left - total);
+          __syncthreads();
+        }
       }
     }
-    __syncthreads();
   }
-  // ascending output: the first pages, the chosen ones, the last ones
+  __syncthreads();
+  // ascending output, SEL_KEYS pages per thread at a time: counts per (round, warp), one scan over them, then the places
   int at = 0;
-  for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
-    const int i = i0 + tid;
-    const bool take = i < n && (i < first || i >= n - last || (rank > 0 && flag[i] == 1));
-    const unsigned ball = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) s_scan[warp] = __popc(ball);
-    __syncthreads();
-    int pos = at + __popc(ball & ((1u << lane) - 1)), total = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) pos += s_scan[w];
-      total += s_scan[w];
+  for (int c0 = 0; c0 < n; c0 += SEL_KEYS * SEL_THREADS) {
+    unsigned ball[SEL_KEYS];
+#pragma unroll
+    for (int j = 0; j < SEL_KEYS; ++j) {
+      const int i = c0 + j * SEL_THREADS + tid;
+      ball[j] = __ballot_sync(0xffffffffu, i < n && (i < first || i >= n - last || (rank > 0 && flag[i] == 1)));
+      if (lane == 0) s_count[j][warp] = __popc(ball[j]);
     }
-    if (take && pos < S) out[pos] = i;
-    at += total;
+    __syncthreads();
+    if (warp == 0) {  // 64 counts, two to a lane
+      int* cnt = &s_count[0][0] + 2 * lane;
+      const int x = cnt[0], y = cnt[1];
+      int inc = x + y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      cnt[0] = inc - x - y;
+      cnt[1] = inc - y;
+      if (lane == 31) s_total = inc;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SEL_KEYS; ++j) {
+      const int pos = at + s_count[j][warp] + __popc(ball[j] & ((1u << lane) - 1));
+      if ((ball[j] >> lane & 1) && pos < S) out[pos] = c0 + j * SEL_THREADS + tid;
+    }
+    at += s_total;
     __syncthreads();
   }
+}
+
+template <int D>
+static int launch_select(const SelectArgs& a, int cluster, cudaStream_t stream) {
+  const int smem = a.cap * 5;
+  Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(select_kernel<D>), SEL_CAP * 5));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(a.t.B) * a.HKV * cluster);
+  cfg.blockDim = dim3(SEL_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(cluster); attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, select_kernel<D>, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the caller's next CUDA call
+    return fail(Q35_ERR_CUDA, "attn.select_pages: %s", cudaGetErrorString(e));
+  }
+  Q35_CUDA_LAUNCH_CHECK("attn.select_pages");
+  return 0;
 }
 
 int run_attn_select_pages(Call& c) {
@@ -535,39 +646,33 @@ int run_attn_select_pages(Call& c) {
   Q35_REQUIRE(D == 64 || D == 128 || D == 256, Q35_ERR_UNSUPPORTED, "%s: head_dim must be 64/128/256", role);
   Q35_REQUIRE(out.s[0] == B && out.s[1] == HKV && S >= 1 && S <= INT_MAX, Q35_ERR_SHAPE, "%s: pages [B, HKV, S]", role);
   Q35_REQUIRE(!keep.present || keep.numel() == 2, Q35_ERR_SHAPE, "%s: keep [2]", role);
-  Q35_REQUIRE(bounds.s[0] >= 1 && bounds.s[0] <= INT_MAX && B * HKV <= INT_MAX / 4, Q35_ERR_SHAPE, "%s: sizes", role);
+  Q35_REQUIRE(bounds.s[0] >= 1 && bounds.s[0] <= INT_MAX && B * HKV <= INT_MAX / 16, Q35_ERR_SHAPE, "%s: sizes", role);
   SelectArgs a{};
   Q35_TRY(get_page_table(c, role, B, 1, bounds.s[0], &a.t));
-  const int64_t E = HKV * int64_t(a.t.n_indices);
+  a.cap = a.t.n_indices < SEL_CAP ? (a.t.n_indices + 15) / 16 * 16 : SEL_CAP;
+  const int64_t E = HKV * int64_t(a.t.n_indices), big = a.t.n_indices > SEL_CAP ? E : 0;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  const int64_t o_sc = take(E * 8), o_zs = take(E * 8), o_zone = take(E * 4), o_flag = take(E);
+  const int64_t o_zs = take(E * 8), o_zone = take(E * 4), o_sc = take(big * 4), o_flag = take(big);
   Q35_TRY(c.workspace(off, &ws));
   if (c.dry || B == 0) return 0;
   Q35_REQUIRE(aligned16(q.p) && aligned16(bounds.p), Q35_ERR_ALIGN, "%s: q and page_bounds must be 16-byte aligned", role);
   a.q = q.as<__nv_bfloat16>(); a.bounds = bounds.as<__nv_bfloat16>();
   a.keep = keep.present ? keep.as<int>() : nullptr;
   a.out = out.as<int>();
-  a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(HQ / HKV); a.D = int(D); a.S = int(S);
+  a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(HQ / HKV); a.S = int(S);
   uint8_t* w = ws.as<uint8_t>();
-  a.score = reinterpret_cast<float2*>(w + o_sc); a.zscore = reinterpret_cast<double*>(w + o_zs);
-  a.zone = reinterpret_cast<int*>(w + o_zone); a.flag = w + o_flag;
-  // CTAs of 64 pages for twice the average sequence; longer ones go around
-  a.gx = int((2 * ((a.t.n_indices + B - 1) / B) + 63) / 64);
-  if (a.gx < 1) a.gx = 1;
-  const int64_t most = INT_MAX / (B * HKV);
-  if (a.gx > most) a.gx = int(most);
-  const dim3 grid(unsigned(B * HKV * a.gx));
-  if (D == 64) launch_pdl(select_score_kernel<64>, grid, dim3(128), 0, c.stream, a);
-  else if (D == 128) launch_pdl(select_score_kernel<128>, grid, dim3(128), 0, c.stream, a);
-  else launch_pdl(select_score_kernel<256>, grid, dim3(128), 0, c.stream, a);
-  Q35_CUDA_LAUNCH_CHECK("attn.select_pages scores");
-  const dim3 rows(unsigned(B * HKV));
-  if (D == 64) launch_pdl(select_choose_kernel<64>, rows, dim3(SEL_THREADS), 0, c.stream, a);
-  else if (D == 128) launch_pdl(select_choose_kernel<128>, rows, dim3(SEL_THREADS), 0, c.stream, a);
-  else launch_pdl(select_choose_kernel<256>, rows, dim3(SEL_THREADS), 0, c.stream, a);
-  Q35_CUDA_LAUNCH_CHECK("attn.select_pages choice");
-  return 0;
+  a.zscore = reinterpret_cast<double*>(w + o_zs);
+  a.zone = reinterpret_cast<int*>(w + o_zone);
+  a.score = reinterpret_cast<float*>(w + o_sc); a.flag = w + o_flag;
+  // four 16-page tiles per CTA for the average sequence (an SM reads a quarter of a megabyte in 3 us), as far as all
+  // clusters run at once, one CTA to an SM (clusters of 8 that have to share SMs do not all find a place: 32 rows of 2048 pages 25.4 us with 4, 28.9 with 8)
+  const int64_t tiles = ((a.t.n_indices + B - 1) / B + 15) / 16;
+  int cluster = 1;
+  while (cluster < 8 && cluster * 4 < tiles && B * HKV * cluster * 2 <= sm_count()) cluster *= 2;
+  if (D == 64) return launch_select<64>(a, cluster, c.stream);
+  if (D == 128) return launch_select<128>(a, cluster, c.stream);
+  return launch_select<256>(a, cluster, c.stream);
 }
 
 }  // namespace q35

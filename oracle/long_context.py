@@ -58,7 +58,7 @@ def page_scores(q, bounds, indptr, indices, last_page_len, b, h):
     out = []
     for g in range(G):
         qg = q[b, h * G + g].double()
-        out.append((qg.clamp(min=0) * hi + qg.clamp(max=0) * lo).sum(-1))
+        out.append(torch.maximum(qg * lo, qg * hi).sum(-1))
     return torch.stack(out).amax(0)
 
 

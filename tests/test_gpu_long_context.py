@@ -169,6 +169,13 @@ def test_select_pages_special_values():
         ref = olc.select_pages(q, bounds, *table, S)
         got = q35.select_pages(gpu(q), gpu(bounds), *gpu(table), S, keep_last=0)
         assert torch.equal(got.cpu(), ref)
+    # keys masked by -inf in one channel: the page's other keys still count, by the sign of the query there
+    q, bounds, table = select_case([60, 60], 1, 128, 3, 6)
+    q[:, :, 7] = torch.tensor([1.0, -1.0]).reshape(2, 1).expand(2, 3).to(torch.bfloat16)
+    page = table[1].long()
+    bounds[page[5:110:4], 0, 0, 7] = float("-inf")
+    for S in (3, 20):
+        assert torch.equal(q35.select_pages(gpu(q), gpu(bounds), *gpu(table), S).cpu(), olc.select_pages(q, bounds, *table, S, 0, 1))
     # a last page without rows is no page
     table[2][0] = 0
     assert torch.equal(q35.select_pages(gpu(q), gpu(bounds), *gpu(table), 8).cpu(), olc.select_pages(q, bounds, *table, 8, 0, 1))
