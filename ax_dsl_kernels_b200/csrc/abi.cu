@@ -204,7 +204,7 @@ static const RoleDef kRoles[] = {
      R"({"in":[["q","bf16","[T,HQ,D]"],["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]"],["qo_indptr","i32","[B+1]"],["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["sm_scale","f32","[1] optional"],["kv_scale","f32","[2,HKV] optional"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes"],["accumulate","i32","[1] optional: bound = add to key_mass instead of storing"],["workspace","u8","[*]"]],"out":[["key_mass","f32","[pages,P,HKV]: the weight the window's queries give to every cached row, causal, summed over queries and the query heads of a KV head"]]})",
      run_attn_key_mass},
     {"attn.evict",
-     R"({"in":[["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["keep","i32","[2] optional: this many first and last rows stay whatever their weight"]],"out":[["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]: kept rows are moved to the sequence's first K"],["key_mass","f32","[pages,P,HKV]: moves with them"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes: moves with them"],["kept","i32","[B,HKV,K]: the kept rows' old positions, ascending, -1 behind"]]})",
+     R"({"in":[["indptr","i32","[B+1]"],["indices","i32","[N]"],["last_page_len","i32","[B]"],["keep","i32","[2] optional: this many first and last rows stay whatever their weight"],["workspace","u8","[*] with tables of more than 49152 rows"]],"out":[["paged_kv_cache","bf16|e4m3","[pages,2,P,HKV,D]: kept rows are moved to the sequence's first K"],["key_mass","f32","[pages,P,HKV]: moves with them"],["paged_kv_scale","bf16","[pages,2,P,HKV] with an int8 cache bound as bytes: moves with them"],["kept","i32","[B,HKV,K]: the kept rows' old positions, ascending, -1 behind"]]})",
      run_attn_evict},
     {"gdn.step",
      R"({"in":[["q","bf16","[B,NK,DK]"],["k","bf16","[B,NK,DK]"],["v","bf16","[B,NV,DV]"],["g","f32","[B,NV]"],["beta","bf16","[B,NV]"],["state_in","f32","[B,NV,DK,DV]"]],"out":[["o","bf16","[B,NV,DV]"],["state_out","f32","[B,NV,DK,DV]"]]})",

@@ -376,6 +376,20 @@ def test_evict(fmt, P, HKV, D, K, first, last):
     assert q35.device_status() == 0
 
 
+def test_evict_from_more_rows_than_fit_on_chip():
+    """60001 rows: the choice works from scratch memory, the moves take many rounds; a whole number of them and not"""
+    import ax_dsl_kernels_b200 as q35
+    for ctx, K in ((60001, 50000), (60001, 3 * 6144), (49152, 49151), (50000, 7)):
+        cache, table, scales, g = make([ctx, 300], 64, 1, 64, "int8", 21)
+        mass = torch.randn((cache.shape[0], 64, 1), generator=g).mul(2).exp()
+        ref, rcache, rmass, rrs = olc.evict(cache, mass, *table, K, 4, 100, scales["row_scale"])
+        gc, gm, gs = gpu(cache), gpu(mass), gpu_scales(scales)
+        kept = q35.evict_keys(gc, gm, *gpu(table), K, keep_first=4, keep_last=100, **gs)
+        assert torch.equal(kept.cpu(), ref)
+        assert torch.equal(gc.cpu(), rcache) and torch.equal(gm.cpu(), rmass) and torch.equal(gs["paged_kv_scale"].cpu(), rrs)
+    assert q35.device_status() == 0
+
+
 @pytest.mark.parametrize("ctx,K", [(5000, 4096), (9000, 1100)])
 def test_evict_ties_and_special_values(ctx, K):
     import ax_dsl_kernels_b200 as q35

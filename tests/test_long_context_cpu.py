@@ -51,6 +51,11 @@ def test_the_contract_accepts_and_describes(role):
     assert _lib.workspace_bytes(role, **empty) >= 0
 
 
+def test_scratch_of_an_eviction_from_a_long_table():
+    t = dict(ROLES["attn.evict"], indices=z(5000, dtype=i32))
+    assert _lib.workspace_bytes("attn.evict", **t) == 5000 * P * HKV * 4
+
+
 def test_scratch_of_the_weights():
     with_mass = dict(ROLES["attn.sparse_decode"], key_mass=MASS)
     assert _lib.workspace_bytes("attn.sparse_decode", **with_mass) == HKV * N * P * 32
