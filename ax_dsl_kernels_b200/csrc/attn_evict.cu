@@ -1,22 +1,21 @@
 // attn.evict: every (sequence, KV head) keeps the min(K, ctx) cached rows with the highest key_mass -- the first and the
 // last ones always, ties to the lower position -- and moves them, in order, to the sequence's first rows, in place.
 //
-// evict_choose, one CTA per (sequence, KV head): the weights once into shared memory as ordered integers, the border by
-// block_kth, then one pass that writes the kept positions in ascending order.
+// evict_choose, one CTA per (sequence, KV head): the weights once into registers as ordered integers, the border by block_kth, then one pass that writes the kept positions in ascending order.
 // evict_move: row j of the result is row kept[j] >= j of the cache.  Bound: HBM, every row that changes place read and
 // written once.
 //
 // In place and in parallel: a cluster takes the kept rows in rounds of consecutive j.  A round stores to rows below its
 // end j1, later rounds load from rows kept[j] >= j >= j1, so loads may run ahead of stores as they like; a round's stores
-// only have to wait until the whole cluster has loaded that round.  A thread owns one row of the round: it asks for its
-// K and V rows with two bulk copies, and a round later, after the cluster's barrier, sends them off with two more.  No
-// data passes through registers, and two rounds' bytes are on their way per CTA.
-// (One CTA per 64-byte column slice, with the rows through registers: 121 us instead of MOVE at 32 x 4000 bf16 rows.)
+// only have to wait until the whole cluster has loaded that round.  A warp owns whole rows of a round: cp.async brings
+// them into its part of the shared memory, and it stores them from there while the cluster's barrier for the next round
+// closes and the one after that is on its way.  (An SM stores 27 bytes a cycle here; loads and barriers hide behind it.)
+// (32 x 4000 bf16 rows: one CTA per 64-byte column slice, without clusters, 121 us; one bulk copy per row and direction,
+// which the copy engine takes one in 16 ns, 66; this MOVE.)
 #include <cooperative_groups.h>
 #include "abi.h"
 #include "attn_pages.cuh"
 #include "block_select.cuh"
-#include "tc_ptx.cuh"
 
 namespace q35 {
 
@@ -32,44 +31,45 @@ struct EvictArgs {
   uint32_t* keys;              // workspace [HKV * n_indices * P], for rows that do not fit the shared memory
   int HKV, K, row_bytes;       // row_bytes of one head
   int cap;                     // rows whose keys fit the shared memory
-  int per_round;               // rows per CTA and round of moves
+  int per_warp;                // rows per warp and round of moves
 };
 
 constexpr int EV_THREADS = 1024;
-constexpr int EV_CAP = 48 * 1024;   // keys in shared memory: 192 KB
-constexpr int EV_U = 8;             // positions per thread on their way together
+constexpr int EV_REGS = 16;         // keys per thread in registers: sequences of up to 16384 rows
+constexpr int EV_CAP = 48 * 1024;   // keys in shared memory, 192 KB, where the registers do not hold them
+constexpr int EV_U = 8;             // positions per thread and round
 
-__global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArgs a) {
-  extern __shared__ __align__(16) uint32_t s_keys[];
-  __shared__ KthScratch<EV_THREADS> s_kth;
-  __shared__ int s_count[EV_U][32], s_total, s_gt[32], s_eq[32];
-  pdl_wait();
-  pdl_launch();
+struct ChooseScratch {
+  KthScratch<EV_THREADS> kth;
+  int count[EV_U][32], total, gt[32], eq[32];
+};
+
+// The choice for one (sequence, KV head) of n > K rows.  Thread t looks at the positions t, t + 1024, ...; key(m) is the
+// key of position m * 1024 + t, set by put(m, key).  M: static number of keys per thread (0: n / 1024, in a loop).
+template <int M, typename Put, typename Key>
+__device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages& sp, int h, int* out, ChooseScratch& s,
+                                             Put put, Key key) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / a.HKV, h = blockIdx.x % a.HKV;
-  const SeqPages sp = seq_pages(a.t, b);
   const int n = sp.ctx, K = a.K, P = a.t.P;
-  int* out = a.kept + size_t(blockIdx.x) * K;
-  if (n <= K) {
-    for (int i = tid; i < K; i += EV_THREADS) out[i] = i < n ? i : -1;
-    return;
-  }
   const int last = a.keep ? min(max(a.keep[1], 0), K) : 0;
   const int first = a.keep ? min(max(a.keep[0], 0), K - last) : 0;
-  const int rank = K - first - last;
-  // keys of the free positions first .. n - last - 1, the forced ones' slots unused
-  uint32_t* keys = n <= a.cap ? s_keys : a.keys + (size_t(a.HKV) * sp.first + size_t(h) * sp.n) * P;
-  const int f0 = first, f1 = n - last;
+  const int rank = K - first - last, f0 = first, f1 = n - last;  // the free rows, of which `rank` are kept
+  const int rounds = M ? M : (n + EV_THREADS - 1) / EV_THREADS;
+  auto is_free = [&](int m) {
+    const int i = m * EV_THREADS + tid;
+    return i >= f0 && i < f1;
+  };
   uint32_t border = 0u;
   int equal = 0;         // how many of the rows that equal the border are kept
   bool ties = false;     // and whether that is not all of them
   if (rank > 0) {
     bool bad = false;
-    for (int i0 = f0 + tid; i0 < f1; i0 += EV_U * EV_THREADS) {
+#pragma unroll
+    for (int m0 = 0; m0 < rounds; m0 += EV_U) {
       int page[EV_U], off[EV_U];
 #pragma unroll
       for (int u = 0; u < EV_U; ++u) {
-        const int i = min(i0 + u * EV_THREADS, f1 - 1), e = a.t.page_of(i);
+        const int i = min((m0 + u) * EV_THREADS + tid, n - 1), e = a.t.page_of(i);
         page[u] = page_or_first(a.t, sp.first + e, bad);
         off[u] = i - e * P;
       }
@@ -78,14 +78,15 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
       for (int u = 0; u < EV_U; ++u) w[u] = a.key_mass[(size_t(page[u]) * P + off[u]) * a.HKV + h];
 #pragma unroll
       for (int u = 0; u < EV_U; ++u)
-        if (i0 + u * EV_THREADS < f1) keys[i0 + u * EV_THREADS] = order_key(w[u]);
+        if (M || (m0 + u) * EV_THREADS + tid < n) put(m0 + u, order_key(w[u]));
     }
     if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
-    // a thread reads only the keys that it wrote itself until the barriers of block_kth are behind it
     auto each = [&](auto f) {
-      for (int i = f0 + tid; i < f1; i += EV_THREADS) f(keys[i]);
+#pragma unroll
+      for (int m = 0; m < rounds; ++m)
+        if (is_free(m)) f(key(m));
     };
-    border = block_kth<EV_THREADS, false>(each, rank, s_kth);
+    border = block_kth<EV_THREADS, false>(each, rank, s.kth);
     int gt = 0, eq = 0;
     each([&](uint32_t k) {
       gt += k > border;
@@ -93,22 +94,22 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
     });
     gt = __reduce_add_sync(0xffffffffu, gt);
     eq = __reduce_add_sync(0xffffffffu, eq);
-    if (lane == 0) { s_gt[warp] = gt; s_eq[warp] = eq; }
+    if (lane == 0) { s.gt[warp] = gt; s.eq[warp] = eq; }
     __syncthreads();
-    equal = rank - __reduce_add_sync(0xffffffffu, s_gt[lane]);
-    ties = equal != __reduce_add_sync(0xffffffffu, s_eq[lane]);
+    equal = rank - __reduce_add_sync(0xffffffffu, s.gt[lane]);
+    ties = equal != __reduce_add_sync(0xffffffffu, s.eq[lane]);
   }
-  // how many flags are set before each of the thread's positions c0 + u * EV_THREADS + tid, and in all (s_total)
+  // how many flags are set before each of the thread's positions of a round, and in all (s.total)
   auto scan = [&](const bool (&flag)[EV_U], int (&at)[EV_U]) {
     unsigned ball[EV_U];
 #pragma unroll
     for (int u = 0; u < EV_U; ++u) {
       ball[u] = __ballot_sync(0xffffffffu, flag[u]);
-      if (lane == 0) s_count[u][warp] = __popc(ball[u]);
+      if (lane == 0) s.count[u][warp] = __popc(ball[u]);
     }
     __syncthreads();
     if (warp == 0) {  // EV_U * 32 counts, EV_U consecutive ones to a lane
-      int* cnt = &s_count[0][0] + EV_U * lane;
+      int* cnt = &s.count[0][0] + EV_U * lane;
       int sum = 0, c[EV_U];
 #pragma unroll
       for (int u = 0; u < EV_U; ++u) { c[u] = sum; sum += cnt[u]; }
@@ -120,21 +121,23 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
       }
 #pragma unroll
       for (int u = 0; u < EV_U; ++u) cnt[u] = inc - sum + c[u];
-      if (lane == 31) s_total = inc;
+      if (lane == 31) s.total = inc;
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u) at[u] = s_count[u][warp] + __popc(ball[u] & ((1u << lane) - 1));
+    for (int u = 0; u < EV_U; ++u) at[u] = s.count[u][warp] + __popc(ball[u] & ((1u << lane) - 1));
   };
   int done = 0, seen = 0;  // kept rows, and rows equal to the border, before this round of positions
-  for (int c0 = 0; c0 < n; c0 += EV_U * EV_THREADS) {
+#pragma unroll
+  for (int m0 = 0; m0 < rounds; m0 += EV_U) {
+    if (m0 * EV_THREADS >= n) break;
     bool take[EV_U], eq[EV_U];
     int at[EV_U];
 #pragma unroll
     for (int u = 0; u < EV_U; ++u) {
-      const int i = c0 + u * EV_THREADS + tid;
-      const bool free_row = i >= f0 && i < f1 && rank > 0;
-      const uint32_t k = free_row ? keys[i] : 0u;
+      const int m = m0 + u, i = m * EV_THREADS + tid;
+      const bool free_row = is_free(m) && rank > 0;
+      const uint32_t k = free_row ? key(m) : 0u;
       eq[u] = free_row && k == border;
       take[u] = i < n && (i < f0 || i >= f1 || (free_row && k > border));
     }
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
       scan(eq, at);
 #pragma unroll
       for (int u = 0; u < EV_U; ++u) eq[u] = eq[u] && seen + at[u] < equal;
-      seen += s_total;
+      seen += s.total;
       __syncthreads();
     }
 #pragma unroll
@@ -150,124 +153,199 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
     scan(take, at);
 #pragma unroll
     for (int u = 0; u < EV_U; ++u)
-      if (take[u] && done + at[u] < K) out[done + at[u]] = c0 + u * EV_THREADS + tid;
-    done += s_total;
+      if (take[u] && done + at[u] < K) out[done + at[u]] = (m0 + u) * EV_THREADS + tid;
+    done += s.total;
     __syncthreads();
   }
 }
 
-constexpr int EM_THREADS = 256;
-constexpr int EM_BUF = 96 * 1024;  // bytes of a round per CTA; two rounds
-
-__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArgs a) {
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ ChooseScratch s;
+  pdl_wait();
+  pdl_launch();
+  const int tid = threadIdx.x, b = blockIdx.x / a.HKV, h = blockIdx.x % a.HKV;
+  const SeqPages sp = seq_pages(a.t, b);
+  int* out = a.kept + size_t(blockIdx.x) * a.K;
+  if (sp.ctx <= a.K) {
+    for (int i = tid; i < a.K; i += EV_THREADS) out[i] = i < sp.ctx ? i : -1;
+    return;
+  }
+  if (sp.ctx <= EV_REGS / 2 * EV_THREADS) {
+    uint32_t k[EV_REGS / 2];
+    evict_choose<EV_REGS / 2>(a, sp, h, out, s, [&](int m, uint32_t x) { k[m] = x; }, [&](int m) { return k[m]; });
+  } else if (sp.ctx <= EV_REGS * EV_THREADS) {
+    uint32_t k[EV_REGS];
+    evict_choose<EV_REGS>(a, sp, h, out, s, [&](int m, uint32_t x) { k[m] = x; }, [&](int m) { return k[m]; });
+  } else {
+    uint32_t* keys = sp.ctx <= a.cap ? s_keys : a.keys + (size_t(a.HKV) * sp.first + size_t(h) * sp.n) * a.t.P;
+    evict_choose<0>(a, sp, h, out, s, [&](int m, uint32_t x) { keys[m * EV_THREADS + tid] = x; },
+                    [&](int m) { return keys[m * EV_THREADS + tid]; });
+  }
 }
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t smem_src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_src), "r"(bytes) : "memory");
-}
 
+constexpr int EM_THREADS = 512, EM_WARPS = EM_THREADS / 32;
+constexpr int EM_BUF = 64 * 1024;  // bytes of a round per CTA; three rounds
+constexpr int EM_PIECES = 8;       // most 16-byte pieces of a row (K and V) per lane: rows of up to 2048 bytes
+
+template <int PL>
 __global__ void __launch_bounds__(EM_THREADS, 1) evict_move_kernel(const EvictArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t s_bar[2];
-  const uint32_t bar = smem_u32(s_bar);
-  const int tid = threadIdx.x;
-  if (tid == 0) {
-    tc::mbar_init(bar, EM_THREADS);
-    tc::mbar_init(bar + 8, EM_THREADS);
-    tc::fence_barrier_init();
-    tc::fence_proxy_async();
-  }
-  __syncthreads();
   pdl_wait();
   pdl_launch();
   cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int NC = int(cluster.num_blocks()), crank = int(cluster.block_rank());
   const int row = blockIdx.x / NC, b = row / a.HKV, h = row % a.HKV;
   const SeqPages sp = seq_pages(a.t, b);
   if (sp.ctx <= a.K) return;  // everything stays where it is: the whole cluster leaves
-  const int n = a.K, P = a.t.P, R = a.per_round;
+  const int n = a.K, P = a.t.P, RW = a.per_warp, R = RW * EM_WARPS;
   const int* kept = a.kept + size_t(row) * a.K;
   const int rounds = (n + NC * R - 1) / (NC * R);
-  const uint32_t mine = smem_u32(smem) + uint32_t(tid) * 2 * a.row_bytes;  // this thread's K and V row in buffer 0
-  // row (position) -> index of its K row among all rows of the cache; -1 where the table names no page
-  auto row_of = [&](int pos) -> int64_t {
-    const int e = a.t.page_of(pos), page = a.t.indices[sp.first + e];
-    return unsigned(page) < unsigned(a.t.num_pages) ? (int64_t(page) * 2 * P + (pos - e * P)) * a.HKV + h : -1;
-  };
-  const int64_t v_rows = int64_t(P) * a.HKV;  // from a K row to its V row
-  auto mass_at = [&](int64_t r) {  // [pages, 2, P, HKV] -> [pages, P, HKV]
+  const int64_t v_rows = int64_t(P) * a.HKV;  // from a K row to its V row, in rows
+  auto mass_at = [&](int64_t r) {             // [pages, 2, P, HKV] -> [pages, P, HKV]
     const int64_t page = r / (2 * v_rows);
     return a.key_mass + (r - page * v_rows);
   };
-  // this thread's row of a round: from where to where, -1 = nothing to do
-  int64_t from[2] = {-1, -1}, to[2] = {-1, -1};
-  float mass[2] = {0.f, 0.f};
-  __nv_bfloat16 ks[2] = {}, vs[2] = {};
-  auto look_up = [&](int i, int64_t& src, int64_t& dst) {
-    const int j = (i * NC + crank) * R + tid;
-    src = dst = -1;
-    if (i < rounds && tid < R && j < n) {
-      const int pos = kept[j];
-      if (pos > j && pos < sp.ctx) {
-        src = row_of(pos);
-        dst = row_of(j);
-        if (src < 0 || dst < 0) {
-          atomicOr(a.t.status, DS_BAD_PAGE);
-          src = dst = -1;
-        }
-      }
+  // Lane l < RW of a warp knows the warp's row l of a round: from where to where, -1 = nothing to do.  The lookups run
+  // ahead of the copies, one step of their chain (kept position, page ids, rows) per round, so that no round waits for
+  // the page table.
+  int64_t from[3] = {-1, -1, -1}, to[3] = {-1, -1, -1};
+  float mass[3] = {0.f, 0.f, 0.f};
+  __nv_bfloat16 ks[3] = {}, vs[3] = {};
+  auto index_of = [&](int i) { return (i * NC + crank) * R + warp * RW + lane; };
+  auto position = [&](int i) -> int {  // kept position of the row of round i, -1 where there is none
+    const int j = index_of(i);
+    return i < rounds && lane < RW && j < n ? kept[j] : -1;
+  };
+  int pos_next, pos_cur, src_page, dst_page;  // position of round i + 3; position and page ids of round i + 2
+  auto ask_pages = [&](int i) {               // page ids of round i, whose position is in pos_cur
+    const int j = index_of(i);
+    src_page = dst_page = -1;
+    if (pos_cur > j && pos_cur < sp.ctx) {
+      src_page = a.t.indices[sp.first + a.t.page_of(pos_cur)];
+      dst_page = a.t.indices[sp.first + a.t.page_of(j)];
+    } else {
+      pos_cur = -1;
     }
   };
-  auto load = [&](int u) {  // u: buffer
-    const uint32_t at = mine + u * EM_BUF, bu = bar + 8 * u;
+  auto row_at = [&](int page, int pos) { return (int64_t(page) * 2 * P + (pos - a.t.page_of(pos) * P)) * a.HKV + h; };
+  auto resolve = [&](int i, int64_t& src, int64_t& dst) {
+    src = dst = -1;
+    if (pos_cur < 0) return;
+    if (unsigned(src_page) < unsigned(a.t.num_pages) && unsigned(dst_page) < unsigned(a.t.num_pages)) {
+      src = row_at(src_page, pos_cur);
+      dst = row_at(dst_page, index_of(i));
+    } else {
+      atomicOr(a.t.status, DS_BAD_PAGE);
+    }
+  };
+  // 16-byte pieces, pp to a row (K, then V): a lane's PL pieces of every row that it takes part in, `rows` rows to an
+  // instruction of the warp where a row has fewer than 32
+  const int pr = a.row_bytes / 16, pp = 2 * pr, rows = pp < 32 ? 32 / pp : 1;
+  const int sub = pp < 32 ? lane / pp : 0, piece0 = pp < 32 ? lane % pp : lane;
+  const int64_t v_off = v_rows * a.row_bytes;
+  int64_t in_cache[PL];
+  bool has[PL];
+#pragma unroll
+  for (int q = 0; q < PL; ++q) {
+    const int p = piece0 + 32 * q;
+    has[q] = sub < rows && p < pp;
+    in_cache[q] = p < pr ? p * 16 : v_off + (p - pr) * 16;
+  }
+  uint8_t* const ring = smem + size_t(warp) * RW * 2 * a.row_bytes;  // the warp's rows in buffer 0
+  auto pieces = [&](int64_t where, auto f) {  // f(address in the cache, offset in the warp's buffer) for every piece
+    const unsigned long long mine = where >= 0 ? reinterpret_cast<unsigned long long>(a.cache) + where * a.row_bytes : 0ull;
+#pragma unroll 4
+    for (int r0 = 0; r0 < RW; r0 += rows) {
+      const int l = r0 + sub;
+      uint8_t* at = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, mine, l & 31));
+      if (l >= RW) at = nullptr;
+#pragma unroll
+      for (int q = 0; q < PL; ++q)
+        if (at && has[q]) f(at + in_cache[q], (l * pp + piece0 + 32 * q) * 16);
+    }
+  };
+  auto load = [&](int i, int u) {  // round i, looked up, into buffer u; then the next lookups
+    resolve(i, from[u], to[u]);
+    __syncwarp();  // the warp has read what the buffer held
+    const uint32_t base = smem_u32(ring) + u * EM_BUF;
+    pieces(from[u], [&](uint8_t* src, int off) { cp_async_16(base + off, src); });
+    cp_async_commit();
     if (from[u] >= 0) {
-      tc::mbar_expect_tx(bu, 2 * a.row_bytes);
-      const uint8_t* src = a.cache + from[u] * a.row_bytes;
-      bulk_load(at, src, a.row_bytes, bu);
-      bulk_load(at + a.row_bytes, src + v_rows * a.row_bytes, a.row_bytes, bu);
       mass[u] = *mass_at(from[u]);
       if (a.row_scale) {
         ks[u] = a.row_scale[from[u]];
         vs[u] = a.row_scale[from[u] + v_rows];
       }
-    } else {
-      tc::mbar_arrive(bu);
     }
+    pos_cur = pos_next;
+    ask_pages(i + 1);
+    pos_next = position(i + 2);
   };
-  auto step = [&](int i, auto cur, auto nxt) {  // cur, nxt: compile-time buffer numbers keep the registers indexed
-    constexpr int U = decltype(cur)::value, V = decltype(nxt)::value;
-    if (i + 1 < rounds) {
-      look_up(i + 1, from[V], to[V]);
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the other buffer has been sent off
-      load(V);
-    }
-    const bool ok = tc::mbar_wait(bar + 8 * U, (i >> 1) & 1);
-    if (!ok) {  // recorded; nothing of this round is stored, and the copies on their way get as long again to land
-      atomicOr(a.t.status, DS_WAIT_TIMEOUT);
-      tc::mbar_wait(bar + 8 * U, (i >> 1) & 1);
-    }
-    cluster.sync();  // the whole cluster has loaded this round
-    if (ok && to[U] >= 0) {
-      const uint32_t at = mine + U * EM_BUF;
-      uint8_t* dst = a.cache + to[U] * a.row_bytes;
-      bulk_store(dst, at, a.row_bytes);
-      bulk_store(dst + v_rows * a.row_bytes, at + a.row_bytes, a.row_bytes);
-      *mass_at(to[U]) = mass[U];
+  auto store = [&](int u) {
+    const uint8_t* base = ring + u * EM_BUF;
+    pieces(to[u], [&](uint8_t* dst, int off) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(base + off);
+    });
+    if (to[u] >= 0) {
+      *mass_at(to[u]) = mass[u];
       if (a.row_scale) {
-        a.row_scale[to[U]] = ks[U];
-        a.row_scale[to[U] + v_rows] = vs[U];
+        a.row_scale[to[u]] = ks[u];
+        a.row_scale[to[u] + v_rows] = vs[u];
       }
     }
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   };
-  look_up(0, from[0], to[0]);
-  load(0);
-  for (int i = 0; i < rounds; i += 2) {
-    step(i, std::integral_constant<int, 0>(), std::integral_constant<int, 1>());
-    if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>(), std::integral_constant<int, 0>());
+  // Round i has arrived: tell the cluster, store round i - 1 meanwhile (the cluster has loaded that one), ask for i + 2.
+  auto step = [&](int i, auto cur, auto prv) {  // compile-time buffer numbers keep the registers indexed
+    cp_async_wait<1>();
+    auto token = cluster.barrier_arrive();
+    if (i > 0) store(decltype(prv)::value);
+    cluster.barrier_wait(std::move(token));
+    load(i + 2, decltype(prv)::value);
+    if (i + 1 == rounds) store(decltype(cur)::value);
+  };
+  pos_cur = position(0);
+  pos_next = position(1);
+  ask_pages(0);
+  load(0, 0);
+  load(1, 1);
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  using B2 = std::integral_constant<int, 2>;
+  for (int i = 0; i < rounds; i += 3) {
+    step(i, B0(), B2());
+    if (i + 1 < rounds) step(i + 1, B1(), B0());
+    if (i + 2 < rounds) step(i + 2, B2(), B1());
   }
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+template <int PL>
+static int launch_evict_move(const EvictArgs& a, int rows, int cluster, cudaStream_t stream) {
+  const void* f = reinterpret_cast<const void*>(evict_move_kernel<PL>);
+  Q35_TRY(ensure_dynamic_smem(f, 3 * EM_BUF));
+  cudaError_t e = cudaSuccess;
+  if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(rows * cluster));
+    cfg.blockDim = dim3(EM_THREADS);
+    cfg.dynamicSmemBytes = 3 * EM_BUF;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster); attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, evict_move_kernel<PL>, a);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the caller's next CUDA call
+    return fail(Q35_ERR_CUDA, "attn.evict: %s", cudaGetErrorString(e));
+  }
+  Q35_CUDA_LAUNCH_CHECK("attn.evict moves");
+  return 0;
 }
 
 int run_attn_evict(Call& c) {
@@ -288,6 +366,8 @@ int run_attn_evict(Call& c) {
   Q35_TRY(get_page_table(c, role, B, kv.P, kv.pages, &a.t));
   a.row_bytes = int(kv.D) * kv.elt();
   Q35_REQUIRE(a.row_bytes % 64 == 0, Q35_ERR_UNSUPPORTED, "%s: a row of a head must be a multiple of 64 bytes", role);
+  Q35_REQUIRE(a.row_bytes <= 256 * EM_PIECES, Q35_ERR_UNSUPPORTED, "%s: a row of a head has %d bytes, at most 2048", role,
+              a.row_bytes);
   Q35_REQUIRE(B * kv.HKV <= INT_MAX / 16, Q35_ERR_SHAPE, "%s: sizes beyond 32 bits", role);
   const int64_t positions = int64_t(a.t.n_indices) * kv.P;  // no sequence has more
   a.cap = int(positions < EV_CAP ? (positions + 31) / 32 * 32 : EV_CAP);
@@ -301,35 +381,17 @@ int run_attn_evict(Call& c) {
   a.keys = ws.present ? ws.as<uint32_t>() : nullptr;
   const int64_t rows = B * kv.HKV;
   Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(evict_choose_kernel), EV_CAP * 4));
-  launch_pdl(evict_choose_kernel, dim3(unsigned(rows)), dim3(EV_THREADS), size_t(a.cap) * 4, c.stream, a);
+  // (no keys in shared memory where every sequence fits the registers)
+  launch_pdl(evict_choose_kernel, dim3(unsigned(rows)), dim3(EV_THREADS),
+             positions > EV_REGS * EV_THREADS ? size_t(a.cap) * 4 : 0, c.stream, a);
   Q35_CUDA_LAUNCH_CHECK("attn.evict choice");
   // as many CTAs per (sequence, KV head) as run at once on an SM each, while a round gives every one of them rows
-  a.per_round = EM_BUF / (2 * a.row_bytes) < EM_THREADS ? EM_BUF / (2 * a.row_bytes) : EM_THREADS;
+  a.per_warp = EM_BUF / (2 * a.row_bytes * EM_WARPS) < 32 ? EM_BUF / (2 * a.row_bytes * EM_WARPS) : 32;
   int cluster = 1;
-  while (cluster < 16 && rows * cluster * 2 <= sm_count() && int64_t(cluster) * a.per_round < a.K) cluster *= 2;
-  const void* f = reinterpret_cast<const void*>(evict_move_kernel);
-  Q35_TRY(ensure_dynamic_smem(f, 2 * EM_BUF));
-  cudaError_t e = cudaSuccess;
-  if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(rows * cluster));
-    cfg.blockDim = dim3(EM_THREADS);
-    cfg.dynamicSmemBytes = 2 * EM_BUF;
-    cfg.stream = c.stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(cluster); attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, evict_move_kernel, a);
-  }
-  if (e != cudaSuccess) {
-    cudaGetLastError();  // reported here, not by the caller's next CUDA call
-    return fail(Q35_ERR_CUDA, "attn.evict: %s", cudaGetErrorString(e));
-  }
-  Q35_CUDA_LAUNCH_CHECK("attn.evict moves");
+  while (cluster < 16 && rows * cluster * 2 <= sm_count() && int64_t(cluster) * a.per_warp * EM_WARPS < a.K) cluster *= 2;
+  Q35_TRY(a.row_bytes <= 256   ? launch_evict_move<1>(a, int(rows), cluster, c.stream)
+          : a.row_bytes <= 512 ? launch_evict_move<2>(a, int(rows), cluster, c.stream)
+                               : launch_evict_move<EM_PIECES>(a, int(rows), cluster, c.stream));
   return 0;
 }
 
