@@ -41,7 +41,7 @@ constexpr int EV_U = 8;             // positions per thread and round
 
 struct ChooseScratch {
   KthScratch<EV_THREADS> kth;
-  int count[EV_U][32], total, gt[32], eq[32];
+  int count[2][EV_U][32], gt[32], eq[32];
 };
 
 // The choice for one (sequence, KV head) of n > K rows.  Thread t looks at the positions t, t + 1024, ...; key(m) is the
@@ -99,33 +99,26 @@ __device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages&
     equal = rank - __reduce_add_sync(0xffffffffu, s.gt[lane]);
     ties = equal != __reduce_add_sync(0xffffffffu, s.eq[lane]);
   }
-  // how many flags are set before each of the thread's positions of a round, and in all (s.total)
+  // how many flags are set before each of the thread's positions of a round; returns how many in all.  Calls alternate
+  // between two sets of counts: one barrier each.
+  int turn = 0;
   auto scan = [&](const bool (&flag)[EV_U], int (&at)[EV_U]) {
+    int (&count)[EV_U][32] = s.count[turn ^= 1];
     unsigned ball[EV_U];
 #pragma unroll
     for (int u = 0; u < EV_U; ++u) {
       ball[u] = __ballot_sync(0xffffffffu, flag[u]);
-      if (lane == 0) s.count[u][warp] = __popc(ball[u]);
+      if (lane == 0) count[u][warp] = __popc(ball[u]);
     }
     __syncthreads();
-    if (warp == 0) {  // EV_U * 32 counts, EV_U consecutive ones to a lane
-      int* cnt = &s.count[0][0] + EV_U * lane;
-      int sum = 0, c[EV_U];
+    int total = 0;
 #pragma unroll
-      for (int u = 0; u < EV_U; ++u) { c[u] = sum; sum += cnt[u]; }
-      int inc = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-#pragma unroll
-      for (int u = 0; u < EV_U; ++u) cnt[u] = inc - sum + c[u];
-      if (lane == 31) s.total = inc;
+    for (int u = 0; u < EV_U; ++u) {
+      const int c = count[u][lane];
+      at[u] = total + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0) + __popc(ball[u] & ((1u << lane) - 1));
+      total += __reduce_add_sync(0xffffffffu, c);
     }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < EV_U; ++u) at[u] = s.count[u][warp] + __popc(ball[u] & ((1u << lane) - 1));
+    return total;
   };
   int done = 0, seen = 0;  // kept rows, and rows equal to the border, before this round of positions
 #pragma unroll
@@ -142,20 +135,18 @@ __device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages&
       take[u] = i < n && (i < f0 || i >= f1 || (free_row && k > border));
     }
     if (ties) {
-      scan(eq, at);
+      const int total = scan(eq, at);
 #pragma unroll
       for (int u = 0; u < EV_U; ++u) eq[u] = eq[u] && seen + at[u] < equal;
-      seen += s.total;
-      __syncthreads();
+      seen += total;
     }
 #pragma unroll
     for (int u = 0; u < EV_U; ++u) take[u] |= eq[u];
-    scan(take, at);
+    const int total = scan(take, at);
 #pragma unroll
     for (int u = 0; u < EV_U; ++u)
       if (take[u] && done + at[u] < K) out[done + at[u]] = (m0 + u) * EV_THREADS + tid;
-    done += s.total;
-    __syncthreads();
+    done += total;
   }
 }
 

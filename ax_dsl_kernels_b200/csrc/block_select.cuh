@@ -7,7 +7,7 @@ namespace q35 {
 // order_key's inverse
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-constexpr int KTH_BINS = 1024, KTH_LIST = 64;
+constexpr int KTH_BITS = 10, KTH_BINS = 1 << KTH_BITS, KTH_LIST = 64;
 
 template <int THREADS>
 struct KthScratch {
@@ -15,7 +15,8 @@ struct KthScratch {
   uint32_t red[2][THREADS / 32];
   int warp_sum[THREADS / 32];
   int count[2][THREADS / 32][8];
-  uint32_t list[KTH_LIST];
+  uint32_t list[KTH_LIST], found;
+  int above[KTH_LIST], same[KTH_LIST];
   int bin, rank, in_bin, listed;
 };
 
@@ -46,6 +47,7 @@ __device__ uint32_t block_kth(Each each, int r, KthScratch<THREADS>& s) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) s.hist[tid + i * THREADS] = 0;
     if (tid == 0) s.listed = 0;
+    if (tid < KTH_LIST) s.above[tid] = s.same[tid] = 0;
     __syncthreads();
     lo = __reduce_min_sync(0xffffffffu, s.red[0][lane % WARPS]);
     hi = __reduce_max_sync(0xffffffffu, s.red[1][lane % WARPS]);
@@ -53,12 +55,12 @@ __device__ uint32_t block_kth(Each each, int r, KthScratch<THREADS>& s) {
   tighten([](uint32_t) { return true; });
   for (int level = 0; level < 3; ++level) {
     if (lo == hi) return lo;
-    const float vlo = key_value(lo), scale = (KTH_BINS - 1) / (BY_VALUE ? key_value(hi) - vlo : float(hi - lo));
-    if (!(scale > 0.f && scale < INFINITY)) break;
     const uint32_t from = lo, to = hi;
-    // rounding keeps the order, so a bin holds an interval of keys
-    auto bin_of = [&](uint32_t k) {
-      return min(KTH_BINS - 1, int((BY_VALUE ? key_value(k) - vlo : float(k - from)) * scale));
+    const float vlo = key_value(lo), scale = (KTH_BINS - 1) / (key_value(hi) - vlo);
+    const int shift = max(0, 32 - KTH_BITS - __clz(hi - lo));  // hi - lo < KTH_BINS << shift
+    if (BY_VALUE && !(scale > 0.f && scale < INFINITY)) break;
+    auto bin_of = [&](uint32_t k) {  // rounding keeps the order, so a bin holds an interval of keys either way
+      return BY_VALUE ? min(KTH_BINS - 1, int((key_value(k) - vlo) * scale)) : int((k - from) >> shift);
     };
     each([&](uint32_t k) {
       if (k >= from && k <= to) atomicAdd(&s.hist[bin_of(k)], 1);
@@ -96,17 +98,23 @@ __device__ uint32_t block_kth(Each each, int r, KthScratch<THREADS>& s) {
         if (k >= from && k <= to && bin_of(k) == bin) s.list[atomicAdd(&s.listed, 1)] = k;
       });
       __syncthreads();
-      uint32_t found = 0u;  // every warp for itself: the key with fewer than rank keys above it and rank at or above it
-      for (int i = lane; i < n; i += 32) {
+      // every key of the list against every other, a part of them per thread: the one with fewer than rank keys above it
+      // and rank at or above it
+      const int i = tid % KTH_LIST;
+      if (i < n) {
         const uint32_t k = s.list[i];
-        int above = 0, equal = 0;
-        for (int j = 0; j < n; ++j) {
+        int above = 0, same = 0;
+        for (int j = tid / KTH_LIST; j < n; j += THREADS / KTH_LIST) {
           above += s.list[j] > k;
-          equal += s.list[j] == k;
+          same += s.list[j] == k;
         }
-        if (above < rank && rank <= above + equal) found = k;
+        if (above) atomicAdd(&s.above[i], above);
+        if (same) atomicAdd(&s.same[i], same);
       }
-      return __reduce_max_sync(0xffffffffu, found);
+      __syncthreads();
+      if (tid < n && s.above[tid] < rank && rank <= s.above[tid] + s.same[tid]) s.found = s.list[tid];
+      __syncthreads();
+      return s.found;
     }
     tighten([&](uint32_t k) { return k >= from && k <= to && bin_of(k) == bin; });
   }
