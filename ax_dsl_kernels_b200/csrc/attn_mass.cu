@@ -6,33 +6,43 @@
 // Two passes over the scores: the first finds lse of every query row, the second adds up columns.  The scores of a pass
 // are not kept: T G values a row are more bytes than the row itself as soon as T G > D / 2.
 //
-// The query rows of a KV head are the G T pairs (token, head), 128 of them to a block, whatever G is.
-// Pass 1 (mass_lse): CTA = 128 query rows x a range of keys; the rows' fragments stay in registers, 64-key tiles stream
-// through shared memory; running maximum and sum per row, merged over the key ranges by mass_merge.
-// Pass 2 (mass_sum): CTA = one 64-key tile, in shared memory once; the blocks of query rows that see it go past.  Every
-// sum has one owner and a fixed order: no atomics.
+// Bound, for long windows: the tensor pipe and the special-function unit alike (a 128 x 128 tile of D = 256 is 1024
+// cycles of MMA and 1024 of exponentials), for short ones the launches and one tile's latency.
+//
+// Both passes are the same pipeline, one CTA per item: a warp of TMA loads, a warp that issues tcgen05.mma (M = N = 128,
+// fp32 accumulators in tensor memory, two of them), and two groups of four warps that read an accumulator each in turn.
+// Pass 1 holds a block of query rows (lanes) and streams 128-key tiles (columns): a thread owns a query row and keeps
+// its running maximum and sum.  Pass 2 holds a 128-key tile (lanes) and streams the blocks of query rows that see it: a
+// thread owns a key and adds up exp2(s - lse).  So every reduction runs along a thread's own columns, every sum has one
+// owner and a fixed order, and nothing is exchanged but the two groups' halves.
+//
+// A block holds the (token, head) pairs of floor(128 / G) tokens, fetched as one 3-D box; the keys come straight from the
+// pages where the cache is bf16 and its pages hold whole swizzle atoms (8 rows), else from a bf16 copy made first.
+#include <cuda.h>
 #include "abi.h"
 #include "attn_pages.cuh"
 #include "kv_formats.cuh"
+#include "tc_host.h"
+#include "tc_ptx.cuh"
 
 namespace q35 {
 
-constexpr int KM_ROWS = 128;   // query rows per block, 16 per warp
-constexpr int KM_KEYS = 64;    // keys per tile
+constexpr int KM_TILE = 128;    // query rows per block, keys per tile
+constexpr int KM_THREADS = 384; // TMA, MMA, two spare warps, two groups of four
 constexpr float KM_LOG2E = 1.4426950408889634f;
 
 struct MassArgs {
   PageTable t;
-  const __nv_bfloat16* q;      // [T_total, HQ, D]
-  const uint8_t* cache;
-  const float* kv_scale;
-  const __nv_bfloat16* row_scale;
   const int* qo_indptr;        // [B + 1]
+  const float* kv_scale;       // E4M3
   const float* sm_scale;       // optional [1]
   float* key_mass;             // [pages, P, HKV]
-  float2* part;                // workspace [splits][HQ T_total]: maximum, sum
-  float* lse;                  // workspace [HQ T_total]: log2 of the sum of 2^score
-  int T_total, HQ, HKV, G, splits, accumulate, q_blocks, key_tiles;
+  float2* part;                // workspace [2 splits][T_total HQ]: maximum, sum
+  float* lse;                  // workspace [T_total HQ]: log2 of the sum of 2^score
+  int T_total, HQ, HKV, G, D, splits, accumulate, e4m3;
+  int tokens;                  // tokens per block of query rows
+  int box_rows;                // rows per TMA box of keys
+  int copied;                  // keys come from the bf16 copy [HKV, n_indices P, D]
 };
 
 // the window of sequence b: tokens q0 .. q0 + T - 1 of q, the first of them at position `first`; T = 0 if there is none
@@ -46,270 +56,413 @@ __device__ __forceinline__ Window window_of(const MassArgs& a, int b, const SeqP
   return {q0, q1 - q0, sp.ctx - (q1 - q0)};
 }
 
-// A tile of 64 rows of K as bf16 in shared memory, from registers loaded one tile ahead.  Chunk ch (8 channels) of row
-// key lies at position ch ^ swz(key): eight lanes that read two rows' four neighbouring chunks hit all 32 banks.
-__device__ __forceinline__ int km_swz(int key) { return (key & 1) << 2 | (key >> 1 & 3); }
-
-template <int D, int KVF>
-struct KTile {
-  static constexpr int CPR = D * (KVF ? 1 : 2) / 16;       // 16-byte chunks of a stored row
-  static constexpr int LD = KM_KEYS * CPR / 256;
-  static constexpr int BYTES = KM_KEYS * D * 2;
-  uint4 v[LD];
-  float sc[LD];
-
-  __device__ __forceinline__ void load(const MassArgs& a, const SeqPages& sp, int kvh, int k0) {
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < LD; ++j) {
-      const int i = threadIdx.x + 256 * j, key = i / CPR, ch = i % CPR, pos = k0 + key;
-      v[j] = make_uint4(0u, 0u, 0u, 0u);  // rows behind the end: zeros (their scores are masked)
-      sc[j] = 0.f;
-      if (pos < sp.ctx) {
-        const int page = page_or_first(a.t, sp.first + pos / a.t.P, bad);
-        const size_t row = (size_t(page) * 2 * a.t.P + pos % a.t.P) * a.HKV + kvh;
-        v[j] = *reinterpret_cast<const uint4*>(a.cache + (row * CPR + ch) * 16);
-        if constexpr (KVF == 2) sc[j] = __bfloat162float(a.row_scale[row]);
-      }
-    }
-    if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
-  }
-  __device__ __forceinline__ void store(uint8_t* tile) const {
-#pragma unroll
-    for (int j = 0; j < LD; ++j) {
-      const int i = threadIdx.x + 256 * j, key = i / CPR, ch = i % CPR;
-      uint4* row = reinterpret_cast<uint4*>(tile + key * D * 2);
-      if constexpr (KVF == 0) {
-        row[ch ^ km_swz(key)] = v[j];
-      } else {
-        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-        uint32_t o[8];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if constexpr (KVF == 2) {
-            o[2 * u] = cvt_s8x2_bf16x2<0, 1>(w[u] ^ 0x80808080u, sc[j], sc[j]);
-            o[2 * u + 1] = cvt_s8x2_bf16x2<2, 3>(w[u] ^ 0x80808080u, sc[j], sc[j]);
-          } else {  // E4M3 -> f16 -> bf16, exact
-            const uint32_t f0 = cvt_kv<0, 1>(w[u]), f1 = cvt_kv<2, 3>(w[u]);
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&f0));
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&f1));
-            o[2 * u] = pack_bf16(x.x, x.y);
-            o[2 * u + 1] = pack_bf16(y.x, y.y);
-          }
-        }
-        row[(2 * ch) ^ km_swz(key)] = make_uint4(o[0], o[1], o[2], o[3]);
-        row[(2 * ch + 1) ^ km_swz(key)] = make_uint4(o[4], o[5], o[6], o[7]);
-      }
-    }
-  }
-};
-
-// A warp's 16 query rows as MMA fragments.  Lane c of a row's four takes channels 8 c .. 8 c + 7 of every 32 (one 16-byte
-// load); the key fragments are read the same way, so both sides agree on the order of k.
-template <int D>
-struct QRows {
-  uint32_t f[D / 32][8];
-  __device__ __forceinline__ void load(const MassArgs& a, const Window& w, int kvh, int row0, int rows) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int m = row0 + r + 8 * half;
-      const bool ok = m < rows;
-      const int tok = ok ? m / a.G : 0, g = ok ? m % a.G : 0;
-      const __nv_bfloat16* p = a.q + (size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + g) * D + 8 * c;
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint4 v = ok ? *reinterpret_cast<const uint4*>(p + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
-        f[j][half] = v.x; f[j][2 + half] = v.y; f[j][4 + half] = v.z; f[j][6 + half] = v.w;
-      }
-    }
-  }
-  // s[nt][0, 1]: row r, keys 8 nt + 2 c, + 1; s[nt][2, 3]: row r + 8
-  __device__ __forceinline__ void scores(const uint8_t* tile, float (&s)[8][4]) const {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const int key = nt * 8 + r;
-        const uint4 k = *reinterpret_cast<const uint4*>(tile + key * D * 2 + (((4 * j + c) ^ km_swz(key)) << 4));
-        mma_bf16_16816(s[nt], f[j][0], f[j][1], f[j][2], f[j][3], k.x, k.y);
-        mma_bf16_16816(s[nt], f[j][4], f[j][5], f[j][6], f[j][7], k.z, k.w);
-      }
-    }
-  }
-};
-
-__device__ __forceinline__ float mass_scale(const MassArgs& a, int kvh, int D, bool e4m3) {
-  const float k_mul = !e4m3 ? 1.f : a.kv_scale ? a.kv_scale[kvh] : 0.125f;
-  return (a.sm_scale ? a.sm_scale[0] : rsqrtf(float(D))) * KM_LOG2E * k_mul;
+__device__ __forceinline__ float mass_scale(const MassArgs& a, int kvh) {
+  const float k_mul = !a.e4m3 ? 1.f : a.kv_scale ? a.kv_scale[kvh] : 0.125f;
+  return (a.sm_scale ? a.sm_scale[0] : rsqrtf(float(a.D))) * KM_LOG2E * k_mul;
 }
 
-template <int D, int KVF>
-__global__ void __launch_bounds__(256, 1) mass_lse_kernel(const MassArgs a) {
-  extern __shared__ __align__(128) uint8_t smem[];
+// ---- the pipeline's own PTX -----------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem], bf16 with fp32 accumulation.  Instruction descriptor: [4,6) 1 = fp32 result, [7,10) and
+// [10,13) 1 = bf16 A and B, [17,23) N >> 3, [24,29) M >> 4
+constexpr uint32_t KM_IDESC = 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(KM_TILE >> 3) << 17 | uint32_t(KM_TILE >> 4) << 24;
+__device__ __forceinline__ void tc_mma_bf16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(ad), "l"(bd), "r"(KM_IDESC), "r"(accumulate) : "memory");
+}
+// this warp's 32 lanes x 32 consecutive columns of fp32 accumulators
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int D>
+struct MassCfg {
+  static constexpr int PANELS = D / 64;                  // 64 channels = the 128 bytes of a swizzled row
+  static constexpr int PANEL = KM_TILE * 128;
+  static constexpr int OPERAND = PANELS * PANEL;         // a block or tile: 64 KB at D = 256
+  static constexpr int STAGES = D == 256 ? 2 : 4;
+  static constexpr int SMEM = 1024 + (1 + STAGES) * OPERAND;
+};
+
+// Which sequence and which of its items an index stands for: sequence b has count(b) items.  Whole warp; n < 0: none.
+template <typename Count>
+__device__ __forceinline__ int2 find_item(int B, int index, Count count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int c = b0 + lane < B ? count(b0 + lane) : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > index);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      return make_int2(b0 + l, index - before - __shfl_sync(0xffffffffu, inc - c, l));
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return make_int2(-1, 0);
+}
+
+template <int D, bool SUM>
+__global__ void __launch_bounds__(KM_THREADS, 1)
+    mass_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const MassArgs a) {
+  using C = MassCfg<D>;
+  using namespace tc;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_bar[2 * C::STAGES + 5];
+  __shared__ uint32_t s_tmem;
+  __shared__ int2 s_item;
+  __shared__ __align__(16) float s_lse[2][2][KM_TILE];  // [group][turn]: minus the lse of the block's query rows
+  __shared__ int s_see[2][2][KM_TILE];                  // and the last key that each of them sees
+  __shared__ float s_half[KM_TILE];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzled tiles start on 1024 bytes
+  const uint32_t held = sbase, ring = sbase + C::OPERAND;
+  const uint32_t bars = smem_u32(s_bar);
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (C::STAGES + s); };
+  auto acc_full = [&](int g) { return bars + 8 * (2 * C::STAGES + g); };
+  auto acc_empty = [&](int g) { return bars + 8 * (2 * C::STAGES + 2 + g); };
+  const uint32_t held_full = bars + 8 * (2 * C::STAGES + 4);
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    for (int g = 0; g < 2; ++g) { mbar_init(acc_full(g), 1); mbar_init(acc_empty(g), 128); }
+    mbar_init(held_full, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&qmap);
+    tma_prefetch_desc(&kmap);
+  }
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int blk = blockIdx.x % a.q_blocks, bh = blockIdx.x / a.q_blocks, b = bh / a.HKV, kvh = bh % a.HKV;
-  const int split = blockIdx.y;
+  if (warp == 0) {
+    const int index = blockIdx.x / a.HKV;
+    const int2 it = find_item(a.t.B, index, [&](int b) {
+      const SeqPages sp = seq_pages(a.t, b);
+      if (SUM) return (sp.ctx + KM_TILE - 1) / KM_TILE;
+      const int T = window_of(a, b, sp).T;
+      return (T + a.tokens - 1) / a.tokens;
+    });
+    if (lane == 0) s_item = it;
+  }
+  // blocks of a.tokens tokens leave the last rows of an operand untouched: zeros there, so that nothing old is NaN
+  const int block_rows = a.tokens * a.G;
+  if (block_rows < KM_TILE) {
+    const int first_op = SUM ? 1 : 0, n_op = SUM ? C::STAGES : 1, per = (KM_TILE - block_rows) * 8;  // 16-byte pieces
+    for (int i = tid; i < n_op * C::PANELS * per; i += KM_THREADS) {
+      const int panel = i / per, at = i % per;
+      asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};"
+                   ::"r"(sbase + first_op * C::OPERAND + panel * C::PANEL + block_rows * 128 + at * 16), "r"(0u));
+    }
+    fence_proxy_async();
+  }
+  __syncthreads();
+  const int b = s_item.x;
+  if (b < 0) return;  // fewer items than the grid's bound
+  if (warp == 2) { tmem_alloc(smem_u32(&s_tmem), 256); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
+  const int kvh = blockIdx.x % a.HKV;
   const SeqPages sp = seq_pages(a.t, b);
   const Window w = window_of(a, b, sp);
-  const int rows = w.T * a.G;
-  const float scale = mass_scale(a, kvh, D, KVF == 1);
-  for (int row0 = blk * KM_ROWS; row0 < rows; row0 += a.q_blocks * KM_ROWS) {
-    // keys that the block's last row sees, cut into a.splits ranges of whole tiles
-    const int last_row = min(row0 + KM_ROWS, rows) - 1, n_keys = w.first + last_row / a.G + 1;
-    const int tiles = (n_keys + KM_KEYS - 1) / KM_KEYS, per = (tiles + a.splits - 1) / a.splits;
-    const int t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-    QRows<D> q;
-    q.load(a, w, kvh, row0 + warp * 16, rows);
-    const int m0 = row0 + warp * 16 + r, m1 = m0 + 8;
-    const int see0 = w.first + m0 / a.G, see1 = w.first + m1 / a.G;  // last key of each row
-    float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    KTile<D, KVF> next;
-    if (t0 < t1) next.load(a, sp, kvh, t0 * KM_KEYS);
-    for (int t = t0; t < t1; ++t) {
-      __syncthreads();
-      next.store(smem);
-      __syncthreads();
-      if (t + 1 < t1) next.load(a, sp, kvh, (t + 1) * KM_KEYS);
-      float s[8][4];
-      q.scores(smem, s);
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = t * KM_KEYS + nt * 8 + 2 * c + (i & 1);
-          s[nt][i] = key <= (i >> 1 ? see1 : see0) ? s[nt][i] * scale : -INFINITY;
-          top[i >> 1] = fmaxf(top[i >> 1], s[nt][i]);
+  const int blocks = (w.T + a.tokens - 1) / a.tokens;
+  // the held operand, and the streamed ones: tiles or blocks number begin .. begin + n - 1
+  const int item = SUM ? s_item.y : blocks - 1 - s_item.y;  // pass 1: the blocks that see most come first
+  int begin, n;
+  if (SUM) {
+    begin = min(blocks, max(0, item * KM_TILE - w.first) / a.tokens);  // the first block that sees the tile's first key
+    n = blocks - begin;
+  } else {
+    const int last = min(w.T, (item + 1) * a.tokens) - 1, tiles = (w.first + last) / KM_TILE + 1;
+    const int per = (tiles + a.splits - 1) / a.splits;
+    begin = min(tiles, int(blockIdx.y) * per);
+    n = min(tiles, begin + per) - begin;
+  }
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA
+    const int boxes = KM_TILE / a.box_rows;
+    // lane l: the row of the tensor map where box l of a tile starts, -1 = behind the end of the sequence
+    auto box_at = [&](int tile) -> int {
+      const int pos = tile * KM_TILE + lane * a.box_rows;
+      if (lane >= boxes || pos >= sp.ctx) return -1;
+      if (a.copied) return kvh * (a.t.n_indices * a.t.P) + sp.first * a.t.P + pos;
+      const int e = a.t.page_of(pos), id = page_at(a.t, sp.first + e);
+      return (id < 0 ? 0 : id) * 2 * a.t.P + (pos - e * a.t.P);
+    };
+    const int x0 = a.copied ? 0 : kvh * D;
+    auto load_keys = [&](int y, uint32_t dst, uint32_t bar) {
+      const int there = __popc(__ballot_sync(0xffffffffu, y >= 0));
+      if (lane == 0) mbar_expect_tx(bar, there * a.box_rows * 128 * C::PANELS);
+      __syncwarp();
+      for (int i0 = 0; i0 < there * C::PANELS; i0 += 32) {
+        const int i = i0 + lane, row = __shfl_sync(0xffffffffu, y, (i / C::PANELS) & 31);
+        if (i < there * C::PANELS)
+          tma_load_2d(dst + (i % C::PANELS) * C::PANEL + (i / C::PANELS) * a.box_rows * 128, &kmap, bar,
+                      x0 + (i % C::PANELS) * 64, row);
+      }
+    };
+    auto load_block = [&](int blk, uint32_t dst, uint32_t bar) {
+      if (lane == 0) mbar_expect_tx(bar, block_rows * 128 * C::PANELS);
+      __syncwarp();
+      if (lane < C::PANELS)
+        tma_load_3d(dst + lane * C::PANEL, &qmap, bar, lane * 64, kvh * a.G, w.q0 + blk * a.tokens);
+    };
+    if (SUM) load_keys(box_at(item), held, held_full);
+    else load_block(item, held, held_full);
+    int y = SUM ? 0 : box_at(begin);
+    for (int t = 0; t < n; ++t) {
+      const int s = t % C::STAGES, next = !SUM && t + 1 < n ? box_at(begin + t + 1) : -1;
+      if (!mbar_wait(empty(s), (t / C::STAGES & 1) ^ 1)) {
+        atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x10);
+        break;
+      }
+      if (SUM) load_block(begin + t, ring + s * C::OPERAND, full(s));
+      else load_keys(y, ring + s * C::OPERAND, full(s));
+      y = next;
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA
+    if (elect_one()) {
+      bool ok = mbar_wait(held_full, 0);
+      if (!ok) atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
+      for (int t = 0; ok && t < n; ++t) {
+        const int s = t % C::STAGES, g = t & 1;
+        if (!mbar_wait(acc_empty(g), (t >> 1 & 1) ^ 1)) {
+          atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x20);
+          break;
         }
+        if (!mbar_wait(full(s), t / C::STAGES & 1)) {
+          atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t streamed = ring + s * C::OPERAND;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        const float mn = fmaxf(mx[h], top[h]), base = mn == -INFINITY ? 0.f : mn;
-        float sum = 0.f;
+        for (int p = 0; p < C::PANELS; ++p)
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) sum += exp2f(s[nt][2 * h] - base) + exp2f(s[nt][2 * h + 1] - base);
-        l[h] = l[h] * exp2f(mx[h] - base) + sum;
-        mx[h] = mn;
+          for (int k = 0; k < 4; ++k)  // 16 channels = 32 bytes of a panel's rows
+            tc_mma_bf16(tmem + g * KM_TILE, smem_desc(held + p * C::PANEL + k * 32, 16, 1024, 2),
+                        smem_desc(streamed + p * C::PANEL + k * 32, 16, 1024, 2), (p | k) != 0);
+        tc_commit(empty(s));
+        tc_commit(acc_full(g));
       }
     }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- accumulators: group g takes every other one
+    const int g = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t acc = tmem + g * KM_TILE + (uint32_t((warp & 3) * 32) << 16);
+    const float scale = mass_scale(a, kvh);
+    // false once a wait has run out (for the whole warp alike); the group's barriers are met all the same
+    bool alive = true;
+    auto wait_acc = [&](int t) {
+      if (alive && !__all_sync(0xffffffffu, mbar_wait(acc_full(g), t >> 1 & 1))) {
+        atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x100);
+        alive = false;
+      }
+      tc_fence_after();
+      return alive;
+    };
+    auto done = [&]() {
+      tc_fence_before();
+      mbar_arrive(acc_empty(g));
+    };
+    if constexpr (!SUM) {
+      const int tok = item * a.tokens + row / a.G;
+      const bool real = row < block_rows && tok < w.T;
+      const int see = w.first + tok, see_min = w.first + item * a.tokens;
+      float m = -INFINITY, l = 0.f;
+      for (int t = g; t < n; t += 2) {
+        const int k0 = (begin + t) * KM_TILE;
+        const bool masked = k0 + KM_TILE - 1 > see_min;  // some row of the block does not see all of the tile
+        if (!wait_acc(t)) break;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int m = h ? m1 : m0;
-      if (c == 0 && m < rows) {
-        const size_t at = size_t(w.q0 + m / a.G) * a.HQ + size_t(kvh) * a.G + m % a.G;
-        a.part[size_t(split) * a.T_total * a.HQ + at] = make_float2(mx[h], l[h]);
+        for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
+          float v[32];
+          tmem_ld_x32(acc + c0, v);
+          if (c0 == KM_TILE - 32) done();
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] *= scale;
+            if (masked && k0 + c0 + i > see) v[i] = -INFINITY;
+            top = fmaxf(top, v[i]);
+          }
+          const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(v[i] - base);
+          l = l * ex2(m - base) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          m = mn;
+        }
+      }
+      if (real) {
+        const size_t rows = size_t(a.T_total) * a.HQ;
+        a.part[(size_t(blockIdx.y) * 2 + g) * rows + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
+            make_float2(m, l);
+      }
+    } else {
+      const int key = item * KM_TILE + row;
+      // the column that this thread fetches the lse of, a turn ahead
+      auto column = [&](int t, float& lse, int& see) {
+        const int tok = (begin + t) * a.tokens + row / a.G;
+        const bool real = t < n && row < block_rows && tok < w.T;
+        lse = real ? -a.lse[size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] : -INFINITY;
+        see = real ? w.first + tok : -1;
+      };
+      float lse;
+      int see;
+      column(g, lse, see);
+      float total = 0.f;
+      for (int t = g; t < n; t += 2) {
+        const int turn = t >> 1 & 1;
+        s_lse[g][turn][row] = lse;
+        s_see[g][turn][row] = see;
+        column(t + 2, lse, see);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
+        // the block's first token sees the whole tile, and its last token is one of the window
+        const int tok0 = (begin + t) * a.tokens;
+        const bool masked = w.first + tok0 < item * KM_TILE + KM_TILE - 1 || tok0 + a.tokens > w.T;
+        if (!wait_acc(t)) continue;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
+          float v[32];
+          tmem_ld_x32(acc + c0, v);
+          if (c0 == KM_TILE - 32) done();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (s_see[g][turn][c0 + i] >= key) sum[i & 3] += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(&s_lse[g][turn][c0 + i]);
+              sum[0] += ex2(fmaf(v[i], scale, x.x));
+              sum[1] += ex2(fmaf(v[i + 1], scale, x.y));
+              sum[2] += ex2(fmaf(v[i + 2], scale, x.z));
+              sum[3] += ex2(fmaf(v[i + 3], scale, x.w));
+            }
+          }
+        }
+        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      }
+      if (g == 1) s_half[row] = total;
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      if (g == 0 && key < sp.ctx) {
+        total += s_half[row];
+        const int e = a.t.page_of(key), page = page_at(a.t, sp.first + e);
+        if (page >= 0) {
+          float* dst = a.key_mass + (size_t(page) * a.t.P + (key - e * a.t.P)) * a.HKV + kvh;
+          *dst = a.accumulate ? *dst + total : total;
+        }
       }
     }
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, 256);
 }
 
-// lse of every query row from its key ranges; a row with no weight at all (every score -inf) gives +inf: no weight
+// lse of every query row from its partial sums; a row with no weight at all (every score -inf) gives +inf: no weight
 __global__ void __launch_bounds__(256) mass_merge_kernel(const MassArgs a) {
   pdl_wait();
   pdl_launch();
   const size_t n = size_t(a.T_total) * a.HQ;
   for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
     float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part[s * n + i].x);
+    for (int s = 0; s < 2 * a.splits; ++s) m = fmaxf(m, a.part[s * n + i].x);
     const float base = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < 2 * a.splits; ++s) {
       const float2 p = a.part[s * n + i];
-      l += p.y * exp2f(p.x - base);
+      l += p.y * ex2(p.x - base);
     }
     a.lse[i] = l == 0.f ? INFINITY : base + log2f(l);
   }
 }
 
-template <int D, int KVF>
-__global__ void __launch_bounds__(256, 1) mass_sum_kernel(const MassArgs a) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_sum[8][KM_KEYS];
+// The K rows of every table entry as bf16 [HKV, n_indices P, D]: one-byte formats (E4M3: the codes' values, exact; int8:
+// bf16(int8 * scale)), and pages that do not hold whole swizzle atoms.  One CTA per entry.
+template <int KVF>
+__global__ void __launch_bounds__(256) mass_copy_kernel(const PageTable t, const uint8_t* cache,
+                                                        const __nv_bfloat16* row_scale, uint4* out, int HKV, int D) {
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-  const int bh = blockIdx.x / a.key_tiles, b = bh / a.HKV, kvh = bh % a.HKV;
-  const SeqPages sp = seq_pages(a.t, b);
-  const Window w = window_of(a, b, sp);
-  const int rows = w.T * a.G;
-  if (rows == 0 && a.accumulate) return;
-  const float scale = mass_scale(a, kvh, D, KVF == 1);
-  for (int tile = blockIdx.x % a.key_tiles; tile * KM_KEYS < sp.ctx; tile += a.key_tiles) {
-    const int k0 = tile * KM_KEYS;
-    __syncthreads();
-    {
-      KTile<D, KVF> k;
-      k.load(a, sp, kvh, k0);
-      k.store(smem);
-    }
-    __syncthreads();
-    float col[8][2];
+  const int e = blockIdx.x;
+  bool bad = false;
+  const int page = page_or_first(t, e, bad);  // an id that is none is recorded by the pass that meets it in a sequence
+  const int cpr = D * (KVF ? 1 : 2) / 16, per_row = HKV * cpr;
+  const uint4* src = reinterpret_cast<const uint4*>(cache) + size_t(page) * 2 * t.P * per_row;
+  const size_t rows = size_t(t.n_indices) * t.P;
+  for (int i = threadIdx.x; i < t.P * per_row; i += 256) {
+    const int r = i / per_row, h = i % per_row / cpr, ch = i % cpr;
+    const uint4 v = src[i];
+    uint4* dst = out + ((size_t(h) * rows + size_t(e) * t.P + r) * D * 2) / 16;
+    if constexpr (KVF == 0) {
+      dst[ch] = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t o[8];
+      float sc = 0.f;
+      if constexpr (KVF == 2) sc = __bfloat162float(row_scale[(size_t(page) * 2 * t.P + r) * HKV + h]);
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt) col[nt][0] = col[nt][1] = 0.f;
-    // the first query row that sees key k0 belongs to token k0 - w.first
-    const int from = max(0, k0 - w.first) * a.G / KM_ROWS * KM_ROWS;
-    for (int row0 = from; row0 < rows; row0 += KM_ROWS) {
-      QRows<D> q;
-      q.load(a, w, kvh, row0 + warp * 16, rows);
-      const int m0 = row0 + warp * 16 + r, m1 = m0 + 8;
-      auto lse = [&](int m) {
-        return m < rows ? a.lse[size_t(w.q0 + m / a.G) * a.HQ + size_t(kvh) * a.G + m % a.G] : INFINITY;
-      };
-      const float l0 = lse(m0), l1 = lse(m1);
-      const int see0 = m0 < rows ? w.first + m0 / a.G : -1, see1 = m1 < rows ? w.first + m1 / a.G : -1;
-      float s[8][4];
-      q.scores(smem, s);
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int key = k0 + nt * 8 + 2 * c + i;
-          if (key <= see0) col[nt][i] += exp2f(s[nt][i] * scale - l0);
-          if (key <= see1) col[nt][i] += exp2f(s[nt][2 + i] * scale - l1);
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (KVF == 2) {
+          o[2 * u] = cvt_s8x2_bf16x2<0, 1>(w[u] ^ 0x80808080u, sc, sc);
+          o[2 * u + 1] = cvt_s8x2_bf16x2<2, 3>(w[u] ^ 0x80808080u, sc, sc);
+        } else {
+          const uint32_t f0 = cvt_kv<0, 1>(w[u]), f1 = cvt_kv<2, 3>(w[u]);
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&f0));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&f1));
+          o[2 * u] = pack_bf16(x.x, x.y);
+          o[2 * u + 1] = pack_bf16(y.x, y.y);
         }
-    }
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) col[nt][i] += __shfl_xor_sync(0xffffffffu, col[nt][i], o);
-        if (r == 0) s_sum[warp][nt * 8 + 2 * c + i] = col[nt][i];
       }
-    __syncthreads();
-    if (threadIdx.x < KM_KEYS && k0 + int(threadIdx.x) < sp.ctx) {
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) sum += s_sum[u][threadIdx.x];
-      const int pos = k0 + threadIdx.x, page = page_at(a.t, sp.first + pos / a.t.P);
-      if (page >= 0) {
-        float* dst = a.key_mass + (size_t(page) * a.t.P + pos % a.t.P) * a.HKV + kvh;
-        *dst = a.accumulate ? *dst + sum : sum;
-      }
+      dst[2 * ch] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[2 * ch + 1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
   }
 }
 
-template <int D, int KVF>
-static int launch_mass(const MassArgs& a, cudaStream_t stream) {
-  const int smem = KTile<D, KVF>::BYTES;
-  const unsigned heads = unsigned(a.t.B) * a.HKV;
-  if (a.T_total > 0) {
-    launch_pdl(mass_lse_kernel<D, KVF>, dim3(heads * a.q_blocks, unsigned(a.splits)), dim3(256), smem, stream, a);
+template <int D>
+static int launch_mass(const MassArgs& a, const CUtensorMap& qmap, const CUtensorMap& kmap, int64_t blocks, int64_t tiles,
+                       cudaStream_t stream) {
+  using C = MassCfg<D>;
+  Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(mass_kernel<D, false>), C::SMEM));
+  Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(mass_kernel<D, true>), C::SMEM));
+  if (blocks) {
+    launch_pdl(mass_kernel<D, false>, dim3(unsigned(blocks * a.HKV), unsigned(a.splits)), dim3(KM_THREADS), C::SMEM, stream,
+               qmap, kmap, a);
     Q35_CUDA_LAUNCH_CHECK("attn.key_mass rows");
-    const int64_t n = int64_t(a.T_total) * a.HQ, blocks = (n + 255) / 256;
-    launch_pdl(mass_merge_kernel, dim3(unsigned(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, a);
+    const int64_t n = (int64_t(a.T_total) * a.HQ + 255) / 256;
+    launch_pdl(mass_merge_kernel, dim3(unsigned(n < 1024 ? n : 1024)), dim3(256), 0, stream, a);
     Q35_CUDA_LAUNCH_CHECK("attn.key_mass merge");
   }
-  launch_pdl(mass_sum_kernel<D, KVF>, dim3(heads * a.key_tiles), dim3(256), smem, stream, a);
+  launch_pdl(mass_kernel<D, true>, dim3(unsigned(tiles * a.HKV)), dim3(KM_THREADS), C::SMEM, stream, qmap, kmap, a);
   Q35_CUDA_LAUNCH_CHECK("attn.key_mass columns");
   return 0;
 }
@@ -328,46 +481,77 @@ int run_attn_key_mass(Call& c) {
   const int64_t T = q.s[0], HQ = q.s[1], D = q.s[2], HKV = kv.HKV, P = kv.P, B = qo.numel() - 1;
   Q35_REQUIRE(kv.D == D && HQ >= 1 && HQ % HKV == 0, Q35_ERR_SHAPE, "%s: head shapes", role);
   Q35_REQUIRE(D == 64 || D == 128 || D == 256, Q35_ERR_UNSUPPORTED, "%s: head_dim must be 64/128/256", role);
+  const int64_t G = HQ / HKV;
+  Q35_REQUIRE(G <= KM_TILE, Q35_ERR_UNSUPPORTED, "%s: at most 128 query heads per KV head (got %lld)", role, (long long)G);
   Q35_REQUIRE(B >= 0 && mass.numel() == kv.pages * P * HKV, Q35_ERR_SHAPE, "%s: qo_indptr [B + 1], key_mass [pages, P, HKV]",
               role);
   Q35_REQUIRE(!scale.present || scale.numel() == 1, Q35_ERR_SHAPE, "%s: sm_scale [1]", role);
-  Q35_REQUIRE(T * HQ <= INT_MAX / 2 && B * HKV <= INT_MAX / 1024, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
   MassArgs a{};
   Q35_TRY(get_page_table(c, role, B, P, kv.pages, &a.t));
-  // pass 1 fills the GPU from (sequence, KV head) x blocks of query rows x ranges of keys
-  const int64_t heads = B * HKV, rows = B ? (T * (HQ / HKV) + B - 1) / B : 0;
-  const int64_t keys = B ? (int64_t(a.t.n_indices) * P + B - 1) / B : 0;
-  int64_t qb = (rows + KM_ROWS - 1) / KM_ROWS;
-  if (qb < 1) qb = 1;
-  const int64_t tiles = (keys + KM_KEYS - 1) / KM_KEYS;
-  int64_t splits = heads ? 2 * sm_count() / (heads * qb) : 1;
-  if (splits > tiles / 2) splits = tiles / 2;
+  const int64_t entries = a.t.n_indices, tokens = KM_TILE / G;
+  // bounds on the items: sequences add a partial one each
+  const int64_t blocks = T ? T / tokens + B : 0, tiles = entries * P / KM_TILE + B;
+  Q35_REQUIRE(T * HQ <= INT_MAX / 2 && B <= INT_MAX / 4 && blocks * HKV <= INT_MAX && tiles * HKV <= INT_MAX,
+              Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
+  // rows per TMA box of keys: the largest power of two that divides a page, whole 8-row swizzle atoms
+  int64_t box = KM_TILE;
+  while (P % box) box /= 2;
+  const bool copied = kv.fmt != 0 || box < 8 || kv.pages * 2 * P > INT_MAX;
+  if (copied) box = KM_TILE;
+  Q35_REQUIRE(!copied || HKV * entries * P <= INT_MAX, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
+  // pass 1 gets about two CTAs per SM from ranges of keys, of at least four tiles each
+  const int64_t items = blocks * HKV, per_seq = B ? tiles / B : 0;
+  int64_t splits = items ? (2 * sm_count() + items - 1) / items : 1;
+  if (splits > per_seq / 4) splits = per_seq / 4;
   if (splits < 1) splits = 1;
-  if (splits > 64) splits = 64;
-  a.q_blocks = int(qb); a.splits = int(splits); a.key_tiles = int(tiles < 1 ? 1 : tiles);
+  if (splits > 32) splits = 32;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  const int64_t o_part = take(splits * T * HQ * 8), o_lse = take(T * HQ * 4);
+  const int64_t o_part = take(2 * splits * T * HQ * 8), o_lse = take(T * HQ * 4),
+                o_copy = take(copied ? HKV * entries * P * D * 2 : 0);
   Q35_TRY(c.workspace(off, &ws));
   if (c.dry || B == 0) return 0;
   Q35_REQUIRE(aligned16(q.p), Q35_ERR_ALIGN, "%s: q must be 16-byte aligned", role);
-  Q35_REQUIRE(heads * a.key_tiles <= INT_MAX && heads * qb <= INT_MAX, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
-  a.q = q.as<__nv_bfloat16>(); a.cache = static_cast<const uint8_t*>(kv.p);
-  a.kv_scale = kv.kv_scale; a.row_scale = kv.row_scale;
+  if (entries == 0) return 0;  // no sequence has a row
   a.qo_indptr = qo.as<int>();
+  a.kv_scale = kv.kv_scale; a.e4m3 = kv.fmt == 1;
   a.sm_scale = scale.present ? scale.as<float>() : nullptr;
   a.key_mass = mass.as<float>();
   uint8_t* w = ws.as<uint8_t>();
   a.part = reinterpret_cast<float2*>(w + o_part);
   a.lse = reinterpret_cast<float*>(w + o_lse);
-  a.T_total = int(T); a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(HQ / HKV);
-  a.accumulate = acc.present;
-#define Q35_MASS(DD) \
-  (kv.fmt == 0 ? launch_mass<DD, 0>(a, c.stream) : kv.fmt == 1 ? launch_mass<DD, 1>(a, c.stream) : launch_mass<DD, 2>(a, c.stream))
-  if (D == 64) return Q35_MASS(64);
-  if (D == 128) return Q35_MASS(128);
-  return Q35_MASS(256);
-#undef Q35_MASS
+  a.T_total = int(T); a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(G); a.D = int(D);
+  a.splits = int(splits); a.accumulate = acc.present; a.tokens = int(tokens); a.box_rows = int(box); a.copied = copied;
+  CUtensorMap qmap, kmap;
+  if (copied) {
+    uint4* out = reinterpret_cast<uint4*>(w + o_copy);
+    const uint8_t* cache = static_cast<const uint8_t*>(kv.p);
+    const dim3 grid{unsigned(entries)};
+    if (kv.fmt == 0)
+      launch_pdl(mass_copy_kernel<0>, grid, dim3(256), 0, c.stream, a.t, cache, kv.row_scale, out, int(HKV), int(D));
+    else if (kv.fmt == 1)
+      launch_pdl(mass_copy_kernel<1>, grid, dim3(256), 0, c.stream, a.t, cache, kv.row_scale, out, int(HKV), int(D));
+    else
+      launch_pdl(mass_copy_kernel<2>, grid, dim3(256), 0, c.stream, a.t, cache, kv.row_scale, out, int(HKV), int(D));
+    Q35_CUDA_LAUNCH_CHECK("attn.key_mass copy");
+    const uint64_t dims[2] = {uint64_t(D), uint64_t(HKV * entries * P)}, strides[1] = {uint64_t(D * 2)};
+    const uint32_t bx[2] = {64, KM_TILE};
+    Q35_TRY(tc_encode_bf16(&kmap, 2, out, dims, strides, bx, "K rows"));
+  } else {
+    const uint64_t dims[2] = {uint64_t(HKV * D), uint64_t(kv.pages * 2 * P)}, strides[1] = {uint64_t(HKV * D * 2)};
+    const uint32_t bx[2] = {64, uint32_t(box)};
+    Q35_TRY(tc_encode_bf16(&kmap, 2, kv.p, dims, strides, bx, "paged_kv_cache"));
+  }
+  if (T) {
+    const uint64_t dims[3] = {uint64_t(D), uint64_t(HQ), uint64_t(T)}, strides[2] = {uint64_t(D * 2), uint64_t(HQ * D * 2)};
+    const uint32_t bx[3] = {64, uint32_t(G), uint32_t(tokens)};
+    Q35_TRY(tc_encode_bf16(&qmap, 3, q.p, dims, strides, bx, "q"));
+  } else {
+    qmap = kmap;  // not read
+  }
+  if (D == 64) return launch_mass<64>(a, qmap, kmap, blocks, tiles, c.stream);
+  if (D == 128) return launch_mass<128>(a, qmap, kmap, blocks, tiles, c.stream);
+  return launch_mass<256>(a, qmap, kmap, blocks, tiles, c.stream);
 }
 
 }  // namespace q35

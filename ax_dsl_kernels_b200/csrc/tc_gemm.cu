@@ -84,6 +84,19 @@ static int encode_map(CUtensorMap* m, bool fp4, const void* base, uint64_t rows,
   return 0;
 }
 
+int tc_encode_bf16(CUtensorMap* m, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  Q35_REQUIRE(fn != nullptr, Q35_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base),
+                        reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides), box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  Q35_REQUIRE(r == CUDA_SUCCESS, Q35_ERR_CUDA, "tensor map for %s rejected by the driver (CUresult %d)", what, int(r));
+  return 0;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // x (bf16) -> two E4M3 terms with UE8M0 block-32 scales: x = hi * 2^eh + lo * 2^el;
 // rows gathered through `src` (destination row -> source row; nullptr = identity).

@@ -12,6 +12,11 @@ namespace q35 {
 int tc_make_map(CUtensorMap* m, bool fp4, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_bytes,
                 uint32_t box_rows, const char* what);
 
+// row-major bf16 tensor of 2 or 3 dims (innermost first; strides in bytes of the dims above it), [box] boxes of 64
+// elements by box[1] by box[2], 128-byte swizzle; not cached
+int tc_encode_bf16(CUtensorMap* m, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, const char* what);
+
 struct TcArgs;
 
 struct TcWeights {            // the two 64-row halves of a tile may come from different matrices (gate / up)
