@@ -10,11 +10,14 @@
 // cycles of MMA and 1024 of exponentials), for short ones the launches and one tile's latency.
 //
 // Both passes are the same pipeline, one CTA per item: a warp of TMA loads, a warp that issues tcgen05.mma (M = N = 128,
-// fp32 accumulators in tensor memory, two of them), and two groups of four warps that read an accumulator each in turn.
+// fp32 accumulators in tensor memory, four of them), and four groups of four warps that read one each in turn.
 // Pass 1 holds a block of query rows (lanes) and streams 128-key tiles (columns): a thread owns a query row and keeps
 // its running maximum and sum.  Pass 2 holds a 128-key tile (lanes) and streams the blocks of query rows that see it: a
 // thread owns a key and adds up exp2(s - lse).  So every reduction runs along a thread's own columns, every sum has one
-// owner and a fixed order, and nothing is exchanged but the two groups' halves.
+// owner and a fixed order, and nothing is exchanged but the groups' partial sums.
+// The groups' arithmetic is what takes longest to keep up: four warps per scheduler hide its latency, two numbers go to
+// an fma or add (f32x2), tiles that every row sees whole have a path without a mask.  (Two groups, a mask for every
+// tile, one number at a time: 273 us instead of GROUPS for 2047 queries over 8192 rows.)
 //
 // A block holds the (token, head) pairs of floor(128 / G) tokens, fetched as one 3-D box; the keys come straight from the
 // pages where the cache is bf16 and its pages hold whole swizzle atoms (8 rows), else from a bf16 copy made first.
@@ -28,7 +31,9 @@
 namespace q35 {
 
 constexpr int KM_TILE = 128;    // query rows per block, keys per tile
-constexpr int KM_THREADS = 384; // TMA, MMA, two spare warps, two groups of four
+constexpr int KM_GROUPS = 4;    // groups of four warps that read accumulators
+constexpr int KM_THREADS = 128 + 128 * KM_GROUPS;  // TMA, MMA, two spare warps, the groups
+constexpr int KM_ACC = 4;       // accumulators of 128 columns: all of tensor memory
 constexpr float KM_LOG2E = 1.4426950408889634f;
 
 struct MassArgs {
@@ -37,7 +42,7 @@ struct MassArgs {
   const float* kv_scale;       // E4M3
   const float* sm_scale;       // optional [1]
   float* key_mass;             // [pages, P, HKV]
-  float2* part;                // workspace [2 splits][T_total HQ]: maximum, sum
+  float2* part;                // workspace [splits][KM_GROUPS][T_total HQ]: maximum, sum
   float* lse;                  // workspace [T_total HQ]: log2 of the sum of 2^score
   int T_total, HQ, HKV, G, D, splits, accumulate, e4m3;
   int tokens;                  // tokens per block of query rows
@@ -93,6 +98,32 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// two fp32 numbers to an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
+  const float2 x = halves(v);
+  return pair(ex2(x.x), ex2(x.y));
+}
+
 template <int D>
 struct MassCfg {
   static constexpr int PANELS = D / 64;                  // 64 channels = the 128 bytes of a swizzled row
@@ -131,24 +162,24 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   using C = MassCfg<D>;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * C::STAGES + 5];
+  __shared__ __align__(8) uint64_t s_bar[2 * C::STAGES + 2 * KM_ACC + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int2 s_item;
-  __shared__ __align__(16) float s_lse[2][2][KM_TILE];  // [group][turn]: minus the lse of the block's query rows
-  __shared__ int s_see[2][2][KM_TILE];                  // and the last key that each of them sees
-  __shared__ float s_half[KM_TILE];
+  __shared__ __align__(16) float s_lse[KM_GROUPS][2][KM_TILE];  // [group][turn]: minus the lse of the block's query rows
+  __shared__ int s_see[KM_GROUPS][2][KM_TILE];                  // and the last key that each of them sees
+  __shared__ float s_sum[KM_GROUPS][KM_TILE];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzled tiles start on 1024 bytes
   const uint32_t held = sbase, ring = sbase + C::OPERAND;
   const uint32_t bars = smem_u32(s_bar);
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (C::STAGES + s); };
-  auto acc_full = [&](int g) { return bars + 8 * (2 * C::STAGES + g); };
-  auto acc_empty = [&](int g) { return bars + 8 * (2 * C::STAGES + 2 + g); };
-  const uint32_t held_full = bars + 8 * (2 * C::STAGES + 4);
+  auto acc_full = [&](int i) { return bars + 8 * (2 * C::STAGES + i); };
+  auto acc_empty = [&](int i) { return bars + 8 * (2 * C::STAGES + KM_ACC + i); };
+  const uint32_t held_full = bars + 8 * (2 * C::STAGES + 2 * KM_ACC);
   if (tid == 0) {
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-    for (int g = 0; g < 2; ++g) { mbar_init(acc_full(g), 1); mbar_init(acc_empty(g), 128); }
+    for (int i = 0; i < KM_ACC; ++i) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 128); }
     mbar_init(held_full, 1);
     fence_barrier_init();
     tma_prefetch_desc(&qmap);
@@ -180,7 +211,7 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   __syncthreads();
   const int b = s_item.x;
   if (b < 0) return;  // fewer items than the grid's bound
-  if (warp == 2) { tmem_alloc(smem_u32(&s_tmem), 256); tmem_relinquish(); }
+  if (warp == 2) { tmem_alloc(smem_u32(&s_tmem), KM_ACC * KM_TILE); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -249,9 +280,12 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
     if (elect_one()) {
       bool ok = mbar_wait(held_full, 0);
       if (!ok) atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
+      // descriptors once: an offset in bytes / 16 is added to their address field (one thread issues all, instruction by
+      // instruction: building a descriptor per MMA took longer than the MMA)
+      const uint64_t held_desc = smem_desc(held, 16, 1024, 2), ring_desc = smem_desc(ring, 16, 1024, 2);
       for (int t = 0; ok && t < n; ++t) {
-        const int s = t % C::STAGES, g = t & 1;
-        if (!mbar_wait(acc_empty(g), (t >> 1 & 1) ^ 1)) {
+        const int s = t % C::STAGES, i = t % KM_ACC;
+        if (!mbar_wait(acc_empty(i), (t / KM_ACC & 1) ^ 1)) {
           atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x20);
           break;
         }
@@ -260,69 +294,90 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t streamed = ring + s * C::OPERAND;
+        const uint64_t streamed = ring_desc + s * (C::OPERAND / 16);
 #pragma unroll
         for (int p = 0; p < C::PANELS; ++p)
 #pragma unroll
           for (int k = 0; k < 4; ++k)  // 16 channels = 32 bytes of a panel's rows
-            tc_mma_bf16(tmem + g * KM_TILE, smem_desc(held + p * C::PANEL + k * 32, 16, 1024, 2),
-                        smem_desc(streamed + p * C::PANEL + k * 32, 16, 1024, 2), (p | k) != 0);
+            tc_mma_bf16(tmem + i * KM_TILE, held_desc + (p * C::PANEL + k * 32) / 16,
+                        streamed + (p * C::PANEL + k * 32) / 16, (p | k) != 0);
         tc_commit(empty(s));
-        tc_commit(acc_full(g));
+        tc_commit(acc_full(i));
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
-    // ---------------------------------------------------------------- accumulators: group g takes every other one
-    const int g = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t acc = tmem + g * KM_TILE + (uint32_t((warp & 3) * 32) << 16);
+    // ---------------------------------------------------------------- accumulators: group g takes every fourth one
+    const int g = (warp - 4) / 4, row = (warp & 3) * 32 + lane;
+    const uint32_t quarter = tmem + (uint32_t((warp & 3) * 32) << 16);
     const float scale = mass_scale(a, kvh);
     // false once a wait has run out (for the whole warp alike); the group's barriers are met all the same
     bool alive = true;
     auto wait_acc = [&](int t) {
-      if (alive && !__all_sync(0xffffffffu, mbar_wait(acc_full(g), t >> 1 & 1))) {
+      if (alive && !__all_sync(0xffffffffu, mbar_wait(acc_full(t % KM_ACC), t / KM_ACC & 1))) {
         atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x100);
         alive = false;
       }
       tc_fence_after();
       return alive;
     };
-    auto done = [&]() {
+    auto done = [&](int t) {
       tc_fence_before();
-      mbar_arrive(acc_empty(g));
+      mbar_arrive(acc_empty(t % KM_ACC));
     };
     if constexpr (!SUM) {
       const int tok = item * a.tokens + row / a.G;
       const bool real = row < block_rows && tok < w.T;
       const int see = w.first + tok, see_min = w.first + item * a.tokens;
       float m = -INFINITY, l = 0.f;
-      for (int t = g; t < n; t += 2) {
+      const uint64_t scale2 = pair(scale, scale);
+      for (int t = g; t < n; t += KM_GROUPS) {
         const int k0 = (begin + t) * KM_TILE;
         const bool masked = k0 + KM_TILE - 1 > see_min;  // some row of the block does not see all of the tile
         if (!wait_acc(t)) break;
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
           float v[32];
-          tmem_ld_x32(acc + c0, v);
-          if (c0 == KM_TILE - 32) done();
-          float top = -INFINITY;
+          tmem_ld_x32(quarter + t % KM_ACC * KM_TILE + c0, v);
+          if (c0 == KM_TILE - 32) done(t);
+          if (masked) {
+            float top = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            v[i] *= scale;
-            if (masked && k0 + c0 + i > see) v[i] = -INFINITY;
-            top = fmaxf(top, v[i]);
+            for (int i = 0; i < 32; ++i) {
+              v[i] = k0 + c0 + i > see ? -INFINITY : v[i] * scale;
+              top = fmaxf(top, v[i]);
+            }
+            const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
+            l *= ex2(m - base);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) l += ex2(v[i] - base);
+            m = mn;
+          } else {
+            float hi[4] = {v[0], v[1], v[2], v[3]}, lo[4] = {v[0], v[1], v[2], v[3]};
+            if (scale >= 0.f) {
+#pragma unroll
+              for (int i = 4; i < 32; ++i) hi[i & 3] = fmaxf(hi[i & 3], v[i]);
+            } else {
+#pragma unroll
+              for (int i = 4; i < 32; ++i) lo[i & 3] = fminf(lo[i & 3], v[i]);
+            }
+            const float top = scale * (scale >= 0.f ? fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3]))
+                                                    : fminf(fminf(lo[0], lo[1]), fminf(lo[2], lo[3])));
+            const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
+            const uint64_t off = pair(-base, -base);
+            uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              sum[i >> 1 & 1] = add2(sum[i >> 1 & 1], ex2_pair(fma2(pair(v[i], v[i + 1]), scale2, off)));
+            const float2 s2 = halves(add2(sum[0], sum[1]));
+            l = l * ex2(m - base) + (s2.x + s2.y);
+            m = mn;
           }
-          const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(v[i] - base);
-          l = l * ex2(m - base) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          m = mn;
         }
       }
       if (real) {
         const size_t rows = size_t(a.T_total) * a.HQ;
-        a.part[(size_t(blockIdx.y) * 2 + g) * rows + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
+        a.part[(size_t(blockIdx.y) * KM_GROUPS + g) * rows + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
             make_float2(m, l);
       }
     } else {
@@ -338,43 +393,44 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
       int see;
       column(g, lse, see);
       float total = 0.f;
-      for (int t = g; t < n; t += 2) {
-        const int turn = t >> 1 & 1;
+      const uint64_t scale2 = pair(scale, scale);
+      for (int t = g; t < n; t += KM_GROUPS) {
+        const int turn = t / KM_GROUPS & 1;
         s_lse[g][turn][row] = lse;
         s_see[g][turn][row] = see;
-        column(t + 2, lse, see);
+        column(t + KM_GROUPS, lse, see);
         asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
-        // the block's first token sees the whole tile, and its last token is one of the window
+        // the block's first token does not see the whole tile, or its last one is behind the window
         const int tok0 = (begin + t) * a.tokens;
         const bool masked = w.first + tok0 < item * KM_TILE + KM_TILE - 1 || tok0 + a.tokens > w.T;
         if (!wait_acc(t)) continue;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+        uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
         for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
           float v[32];
-          tmem_ld_x32(acc + c0, v);
-          if (c0 == KM_TILE - 32) done();
+          tmem_ld_x32(quarter + t % KM_ACC * KM_TILE + c0, v);
+          if (c0 == KM_TILE - 32) done(t);
           if (masked) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (s_see[g][turn][c0 + i] >= key) sum[i & 3] += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
+              if (s_see[g][turn][c0 + i] >= key) total += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(&s_lse[g][turn][c0 + i]);
-              sum[0] += ex2(fmaf(v[i], scale, x.x));
-              sum[1] += ex2(fmaf(v[i + 1], scale, x.y));
-              sum[2] += ex2(fmaf(v[i + 2], scale, x.z));
-              sum[3] += ex2(fmaf(v[i + 3], scale, x.w));
+              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&s_lse[g][turn][c0 + i]);
+              sum[0] = add2(sum[0], ex2_pair(fma2(pair(v[i], v[i + 1]), scale2, x.x)));
+              sum[1] = add2(sum[1], ex2_pair(fma2(pair(v[i + 2], v[i + 3]), scale2, x.y)));
             }
           }
         }
-        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 s2 = halves(add2(sum[0], sum[1]));
+        total += s2.x + s2.y;
       }
-      if (g == 1) s_half[row] = total;
-      asm volatile("bar.sync 3, 256;" ::: "memory");
+      s_sum[g][row] = total;
+      asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
       if (g == 0 && key < sp.ctx) {
-        total += s_half[row];
+#pragma unroll
+        for (int i = 1; i < KM_GROUPS; ++i) total += s_sum[i][row];
         const int e = a.t.page_of(key), page = page_at(a.t, sp.first + e);
         if (page >= 0) {
           float* dst = a.key_mass + (size_t(page) * a.t.P + (key - e * a.t.P)) * a.HKV + kvh;
@@ -385,7 +441,7 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 2) tmem_dealloc(tmem, 256);
+  if (warp == 2) tmem_dealloc(tmem, KM_ACC * KM_TILE);
 }
 
 // lse of every query row from its partial sums; a row with no weight at all (every score -inf) gives +inf: no weight
@@ -395,9 +451,9 @@ __global__ void __launch_bounds__(256) mass_merge_kernel(const MassArgs a) {
   const size_t n = size_t(a.T_total) * a.HQ;
   for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
     float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < 2 * a.splits; ++s) m = fmaxf(m, a.part[s * n + i].x);
+    for (int s = 0; s < KM_GROUPS * a.splits; ++s) m = fmaxf(m, a.part[s * n + i].x);
     const float base = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < 2 * a.splits; ++s) {
+    for (int s = 0; s < KM_GROUPS * a.splits; ++s) {
       const float2 p = a.part[s * n + i];
       l += p.y * ex2(p.x - base);
     }
@@ -507,7 +563,7 @@ int run_attn_key_mass(Call& c) {
   if (splits > 32) splits = 32;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  const int64_t o_part = take(2 * splits * T * HQ * 8), o_lse = take(T * HQ * 4),
+  const int64_t o_part = take(KM_GROUPS * splits * T * HQ * 8), o_lse = take(T * HQ * 4),
                 o_copy = take(copied ? HKV * entries * P * D * 2 : 0);
   Q35_TRY(c.workspace(off, &ws));
   if (c.dry || B == 0) return 0;
