@@ -42,8 +42,7 @@ struct MassArgs {
   const float* kv_scale;       // E4M3
   const float* sm_scale;       // optional [1]
   float* key_mass;             // [pages, P, HKV]
-  float2* part;                // workspace [splits][KM_GROUPS][T_total HQ]: maximum, sum
-  float* lse;                  // workspace [T_total HQ]: log2 of the sum of 2^score
+  float2* part;                // workspace [splits][T_total HQ]: maximum and sum of a query row over a range of keys
   int T_total, HQ, HKV, G, D, splits, accumulate, e4m3;
   int tokens;                  // tokens per block of query rows
   int box_rows;                // rows per TMA box of keys
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   __shared__ int2 s_item;
   __shared__ __align__(16) float s_lse[KM_GROUPS][2][KM_TILE];  // [group][turn]: minus the lse of the block's query rows
   __shared__ int s_see[KM_GROUPS][2][KM_TILE];                  // and the last key that each of them sees
-  __shared__ float s_sum[KM_GROUPS][KM_TILE];
+  __shared__ float s_sum[2 * KM_GROUPS][KM_TILE];               // the groups' sums (pass 1: maxima, then sums)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzled tiles start on 1024 bytes
   const uint32_t held = sbase, ring = sbase + C::OPERAND;
@@ -375,19 +374,46 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
           }
         }
       }
-      if (real) {
-        const size_t rows = size_t(a.T_total) * a.HQ;
-        a.part[(size_t(blockIdx.y) * KM_GROUPS + g) * rows + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
+      s_sum[g][row] = m;
+      s_sum[KM_GROUPS + g][row] = l;
+      asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
+      if (g == 0 && real) {
+#pragma unroll
+        for (int i = 1; i < KM_GROUPS; ++i) m = fmaxf(m, s_sum[i][row]);
+        const float base = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < KM_GROUPS; ++i) l += s_sum[KM_GROUPS + i][row] * ex2(s_sum[i][row] - base);
+        a.part[size_t(blockIdx.y) * a.T_total * a.HQ + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
             make_float2(m, l);
       }
     } else {
       const int key = item * KM_TILE + row;
-      // the column that this thread fetches the lse of, a turn ahead
+      // the column whose lse this thread finds, a turn ahead, from the key ranges' maxima and sums; a query row with no
+      // weight at all (every score -inf) and a column that stands for none get an infinite one: no weight
+      const size_t rows = size_t(a.T_total) * a.HQ;
       auto column = [&](int t, float& lse, int& see) {
         const int tok = (begin + t) * a.tokens + row / a.G;
         const bool real = t < n && row < block_rows && tok < w.T;
-        lse = real ? -a.lse[size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] : -INFINITY;
+        lse = -INFINITY;
         see = real ? w.first + tok : -1;
+        if (!real) return;
+        const float2* p = a.part + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G;
+        float m = -INFINITY, l = 0.f;
+        for (int s0 = 0; s0 < a.splits; s0 += 8) {
+          float2 x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[u] = s0 + u < a.splits ? p[(s0 + u) * rows] : make_float2(-INFINITY, 0.f);
+          float top = m;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+          const float base = top == -INFINITY ? 0.f : top;
+          l *= ex2(m - base);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) l += x[u].y * ex2(x[u].x - base);
+          m = top;
+        }
+        if (l != 0.f) lse = -((m == -INFINITY ? 0.f : m) + log2f(l));
       };
       float lse;
       int see;
@@ -444,23 +470,6 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   if (warp == 2) tmem_dealloc(tmem, KM_ACC * KM_TILE);
 }
 
-// lse of every query row from its partial sums; a row with no weight at all (every score -inf) gives +inf: no weight
-__global__ void __launch_bounds__(256) mass_merge_kernel(const MassArgs a) {
-  pdl_wait();
-  pdl_launch();
-  const size_t n = size_t(a.T_total) * a.HQ;
-  for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) {
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < KM_GROUPS * a.splits; ++s) m = fmaxf(m, a.part[s * n + i].x);
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int s = 0; s < KM_GROUPS * a.splits; ++s) {
-      const float2 p = a.part[s * n + i];
-      l += p.y * ex2(p.x - base);
-    }
-    a.lse[i] = l == 0.f ? INFINITY : base + log2f(l);
-  }
-}
-
 // The K rows of every table entry as bf16 [HKV, n_indices P, D]: one-byte formats (E4M3: the codes' values, exact; int8:
 // bf16(int8 * scale)), and pages that do not hold whole swizzle atoms.  One CTA per entry.
 template <int KVF>
@@ -514,9 +523,6 @@ static int launch_mass(const MassArgs& a, const CUtensorMap& qmap, const CUtenso
     launch_pdl(mass_kernel<D, false>, dim3(unsigned(blocks * a.HKV), unsigned(a.splits)), dim3(KM_THREADS), C::SMEM, stream,
                qmap, kmap, a);
     Q35_CUDA_LAUNCH_CHECK("attn.key_mass rows");
-    const int64_t n = (int64_t(a.T_total) * a.HQ + 255) / 256;
-    launch_pdl(mass_merge_kernel, dim3(unsigned(n < 1024 ? n : 1024)), dim3(256), 0, stream, a);
-    Q35_CUDA_LAUNCH_CHECK("attn.key_mass merge");
   }
   launch_pdl(mass_kernel<D, true>, dim3(unsigned(tiles * a.HKV)), dim3(KM_THREADS), C::SMEM, stream, qmap, kmap, a);
   Q35_CUDA_LAUNCH_CHECK("attn.key_mass columns");
@@ -563,8 +569,7 @@ int run_attn_key_mass(Call& c) {
   if (splits > 32) splits = 32;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
-  const int64_t o_part = take(KM_GROUPS * splits * T * HQ * 8), o_lse = take(T * HQ * 4),
-                o_copy = take(copied ? HKV * entries * P * D * 2 : 0);
+  const int64_t o_part = take(splits * T * HQ * 8), o_copy = take(copied ? HKV * entries * P * D * 2 : 0);
   Q35_TRY(c.workspace(off, &ws));
   if (c.dry || B == 0) return 0;
   Q35_REQUIRE(aligned16(q.p), Q35_ERR_ALIGN, "%s: q must be 16-byte aligned", role);
@@ -575,7 +580,6 @@ int run_attn_key_mass(Call& c) {
   a.key_mass = mass.as<float>();
   uint8_t* w = ws.as<uint8_t>();
   a.part = reinterpret_cast<float2*>(w + o_part);
-  a.lse = reinterpret_cast<float*>(w + o_lse);
   a.T_total = int(T); a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(G); a.D = int(D);
   a.splits = int(splits); a.accumulate = acc.present; a.tokens = int(tokens); a.box_rows = int(box); a.copied = copied;
   CUtensorMap qmap, kmap;
