@@ -114,6 +114,16 @@ def _workspace(dev, nbytes, stream):
     return got[1]
 
 
+def _scratch(dev, nbytes, stream):
+    """(address, owner) of a call's workspace.  While a CUDA graph is being captured it comes from the graph's own memory:
+    a graph must not hold the address of a buffer that a later, larger call replaces, nor share one with another graph
+    that may be replayed beside it."""
+    if torch.cuda.is_current_stream_capturing():
+        own = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
+        return own.data_ptr(), own
+    return _workspace(dev, nbytes, stream), None
+
+
 class _Plan:
     """What a call signature (role, names, dtypes, shapes) always binds: the IO table with everything but the pointers,
     and the scratch the role needs.  `workspace`, when the role needs it and the caller brings none, is the last entry."""
@@ -136,12 +146,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def run(role, stream=None, **tensors):
-    """q35_run(role, ...) with the given tensors bound by name; a `workspace` is added when the role needs one.
-
-    The IO table of a signature is built (and checked) once and copied per call.  While a CUDA graph is being captured
-    the workspace comes from the graph's own memory: a graph must not hold the address of a buffer that a later, larger
-    call replaces, nor share one with another graph that may be replayed beside it."""
+def run_checked(role, stream=None, **tensors):
+    """run() in Python: every check by name, for the calls that binding/bind.cc passes on and where it is not built.  The
+    IO table of a signature is built once and copied per call."""
     L = lib()
     ts = tensors.values()
     devices = {t.get_device() for t in ts}
@@ -162,11 +169,8 @@ def run(role, stream=None, **tensors):
     if stream is None:
         stream = _raw_stream(dev)
     if plan.need:
-        if torch.cuda.is_current_stream_capturing():
-            own = torch.empty(plan.need, dtype=torch.uint8, device=torch.device("cuda", dev))
-            ptrs.append(own.data_ptr())
-        else:
-            ptrs.append(_workspace(dev, plan.need, stream))
+        own = _scratch(dev, plan.need, stream)
+        ptrs.append(own[0])
     table = plan.words.from_buffer_copy(plan.bytes)
     i = _PTR_WORD
     for p in ptrs:
@@ -177,6 +181,31 @@ def run(role, stream=None, **tensors):
     else:
         with torch.cuda.device(dev):
             _check(L.q35_run(plan.role, table, plan.n, stream))
+
+
+_fast = None
+
+
+def _fast_run():
+    """binding/bind.cc's run, or run_checked where it was not built for this torch"""
+    try:
+        from . import _bind
+    except ImportError:
+        return run_checked
+    L = lib()
+    address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+    _bind.init(address(L.q35_run), address(L.q35_workspace_bytes), run_checked, _scratch, _check)
+    return _bind.run
+
+
+def run(role, stream=None, **tensors):
+    """q35_run(role, ...) with the given tensors bound by name; a `workspace` is added when the role needs one.  The
+    tensors are contiguous and on one GPU; the call goes to its current stream, or to the one given (a cudaStream_t as an
+    integer).  The first call replaces this function in the module by its fast form."""
+    global _fast, run
+    if _fast is None:
+        _fast = run = _fast_run()
+    return _fast(role, stream, **tensors)
 
 
 def io_table(role):

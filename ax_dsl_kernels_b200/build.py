@@ -1,5 +1,6 @@
 """Builds csrc/*.cu into libq35b200.so (in-tree, sm_100a only) with nvcc, and the native by-name runner
-runner/q35run.cc (plain C++ against the library's C ABI and the CUDA runtime) into ./q35run.
+runner/q35run.cc (plain C++ against the library's C ABI and the CUDA runtime) into ./q35run, and the Python binding's
+fast path binding/bind.cc (against the installed torch) into ./_bind.so.
 
     python -m ax_dsl_kernels_b200.build [--force]
 """
@@ -13,6 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libq35b200.so")
 RUNNER = os.path.join(HERE, "q35run")
 RUNNER_SRC = os.path.join(HERE, "runner", "q35run.cc")
+BIND = os.path.join(HERE, "_bind.so")
+BIND_SRC = os.path.join(HERE, "binding", "bind.cc")
 OBJ = os.path.join(HERE, "build")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -39,6 +42,21 @@ def _compile(src):
     return obj
 
 
+def _build_binding():
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    inc = [*include_paths(), sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    lib = [d for p in library_paths() for d in ("-L", p, "-Wl,-rpath," + p)]
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[a for d in inc for a in ("-isystem", d)], BIND_SRC, "-o", BIND, *lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"binding build failed:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
@@ -60,6 +78,8 @@ def build(force=False, verbose=False):
                             "$ORIGIN"], capture_output=True, text=True)
         if r.returncode:
             raise RuntimeError(f"runner build failed:\n{r.stdout}\n{r.stderr}")
+    if force or _stale(BIND, [BIND_SRC, headers[-1]]):
+        _build_binding()
     return LIB
 
 

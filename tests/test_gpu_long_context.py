@@ -540,6 +540,32 @@ def test_a_captured_graph_keeps_its_own_scratch():
     assert torch.equal(out, want) and torch.equal(gm, gm2)
 
 
+def test_both_host_paths_issue_the_same_call():
+    """the binding's fast path and the checked one, on a stream given by its handle too; what neither takes is refused"""
+    import ax_dsl_kernels_b200 as q35
+    from ax_dsl_kernels_b200 import _lib
+    cache, table, _, g = make([700, 90], 64, 2, 128, "bf16", 22)
+    gt, gc, q = dict(zip(("indptr", "indices", "last_page_len"), gpu(table))), gpu(cache), gpu(q_rows(2, 16, 128, g, 2.0))
+    got = []
+    side = torch.cuda.Stream()
+    for run, kw in ((_lib.run_checked, {}), (_lib.run, {}), (_lib.run, dict(stream=side.cuda_stream))):
+        out, gm = torch.empty_like(q), torch.zeros((cache.shape[0], 64, 2), device="cuda")
+        torch.cuda.synchronize()
+        run("attn.sparse_decode", q=q, paged_kv_cache=gc, **gt, out=out, key_mass=gm, **kw)
+        torch.cuda.synchronize()
+        got.append((out, gm))
+    for out, gm in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(gm, got[0][1])
+    bad = dict(q=q, paged_kv_cache=gc, **gt, out=torch.empty_like(q))
+    for run in (_lib.run_checked, _lib.run):
+        for change, error in ((dict(q=q.cpu()), ValueError), (dict(q=q.transpose(0, 1)), ValueError), (dict(out=3), Exception),
+                              (dict(q=q.double()), TypeError), (dict(out=q[:1].clone()), q35.Q35Error)):
+            with pytest.raises(error):
+                run("attn.sparse_decode", **dict(bad, **change))
+        with pytest.raises(q35.Q35Error):
+            run("attn.no_such_role", q=q)
+
+
 # ---------------------------------------------------------------------------------------------------- bad tables
 def test_bad_tables_are_recorded_and_touch_nothing():
     """page ids outside the cache, ranges outside the table, lists of pages that are not ascending"""
