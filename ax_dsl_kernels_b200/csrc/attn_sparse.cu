@@ -62,10 +62,12 @@ struct SparseCfg {
   static constexpr int PART = WARPS * SP_G * D * 4;     // the warps' output partials reuse the ring
   static constexpr int SMEM = RING > PART ? RING : PART;
   static constexpr int LD = SP_KEYS * CPR / 32;         // chunks per lane and half step
+  // CTAs per SM: as the ring and the accumulators' registers (up to 255, 170, 128 a thread) allow
+  static constexpr int CTAS = D == 256 ? (BYTE ? 2 : 1) : D == 128 ? (BYTE ? 3 : 2) : 4;
 };
 
 template <int D, int KVF>
-__global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, 1) sparse_decode_kernel(const SparseArgs a) {
+__global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KVF>::CTAS) sparse_decode_kernel(const SparseArgs a) {
   using C = SparseCfg<D, KVF>;
   constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -593,10 +595,10 @@ static int launch_sparse(const SparseArgs& a, cudaStream_t stream) {
   const void* f = reinterpret_cast<const void*>(sparse_decode_kernel<D, KVF>);
   // the 48 KB that need no opt-in hold the static arrays too: head_dim 64 is above them with exactly 48 KB of ring
   Q35_TRY(ensure_dynamic_smem(f, C::SMEM > 49 * 1024 ? C::SMEM : 49 * 1024));
-  const int resident = 200 * 1024 / C::SMEM < 1 ? 1 : 200 * 1024 / C::SMEM;
   const int64_t rows = int64_t(a.t.B) * a.HKV;
   const int64_t keys = int64_t(a.t.P) * (a.pages ? a.S : (a.t.n_indices + a.t.B - 1) / a.t.B);
-  const int cluster = sparse_cluster(rows, (keys + SP_KEYS - 1) / SP_KEYS, (resident < 2 ? 1 : 2) * sm_count(), a.pages != nullptr);
+  const int cluster = sparse_cluster(rows, (keys + SP_KEYS - 1) / SP_KEYS, C::CTAS * sm_count(),
+                                     a.pages != nullptr);
   cudaError_t e = cudaSuccess;
   if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) {
