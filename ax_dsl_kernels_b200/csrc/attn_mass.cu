@@ -132,29 +132,6 @@ struct MassCfg {
   static constexpr int SMEM = 1024 + (1 + STAGES) * OPERAND;
 };
 
-// Which sequence and which of its items an index stands for: sequence b has count(b) items.  Whole warp; n < 0: none.
-template <typename Count>
-__device__ __forceinline__ int2 find_item(int B, int index, Count count) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < B; b0 += 32) {
-    const int c = b0 + lane < B ? count(b0 + lane) : 0;
-    int inc = c;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > index);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      return make_int2(b0 + l, index - before - __shfl_sync(0xffffffffu, inc - c, l));
-    }
-    before += __shfl_sync(0xffffffffu, inc, 31);
-  }
-  return make_int2(-1, 0);
-}
-
 template <int D, bool SUM>
 __global__ void __launch_bounds__(KM_THREADS, 1)
     mass_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const MassArgs a) {

@@ -69,6 +69,29 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Which sequence, and which of its items, an index stands for when sequence b has count(b) items (whole warp); -1: none
+template <typename Count>
+__device__ __forceinline__ int2 find_item(int B, int index, Count count) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int c = b0 + lane < B ? count(b0 + lane) : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > index);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      return make_int2(b0 + l, index - before - __shfl_sync(0xffffffffu, inc - c, l));
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return make_int2(-1, 0);
+}
+
 struct KvCache {
   const void* p = nullptr;                    // [pages, 2, P, HKV, D]
   int fmt = 0;                                // 0 bf16, 1 E4M3, 2 int8 with row scales

@@ -41,7 +41,9 @@ struct SparseArgs {
   __nv_bfloat16* out;              // [B, HQ, D]
   float* key_mass;                 // optional [pages, P, HKV]
   float* scores;                   // workspace, with key_mass: 8 floats per row
+  float* part_o; float* part_ml;   // workspace of the flat form: [rows + n_cta][8][D], [rows + n_cta][16]
   int HQ, HKV, G, S;
+  int n_cta, chunks;               // flat form: CTAs of the first kernel, CTAs per (sequence, KV head) of the second
 };
 
 // KVF: 0 bf16, 1 E4M3, 2 int8 rows with scales.
@@ -66,7 +68,67 @@ struct SparseCfg {
   static constexpr int CTAS = D == 256 ? (BYTE ? 2 : 1) : D == 128 ? (BYTE ? 3 : 2) : 4;
 };
 
-template <int D, int KVF>
+// key_mass += weights of the rows k_begin .. k_end - 1 of a (sequence, KV head), from their scores and the heads' final
+// maxima and inverse sums; `lifted`: how many times the sums are larger than what a score stands for.
+template <int THREADS>
+__device__ __forceinline__ void add_weights(const SparseArgs& a, const SeqPages& sp, const int* pages, int kvh,
+                                            const float* scores, int k_begin, int k_end, const float* s_top,
+                                            const float* s_inv, float lifted) {
+  // Four rows of every thread on their way together, no branch between them: rows behind the end read the last row's
+  // scores and add nothing.  (One or two warps per scheduler: what counts here is the number of instructions per row.)
+  constexpr int U = 4;
+  float top[SP_G], inv[SP_G];
+#pragma unroll
+  for (int g = 0; g < SP_G; ++g) {
+    top[g] = s_top[g];
+    inv[g] = g < a.G ? s_inv[g] * lifted : 0.f;
+  }
+  for (int k0 = k_begin + int(threadIdx.x); k0 < k_end; k0 += U * THREADS) {
+    float4 lo[U], hi[U];
+    int page[U], off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = min(k0 + u * THREADS, k_end - 1), e = a.t.page_of(k);
+      lo[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G);
+      hi[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G + 4);
+      page[u] = a.t.indices[sp.first + (pages ? pages[e] : e)];  // no page: recorded by the step that read the row
+      off[u] = k - e * a.t.P;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float s[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+      float w = 0.f;
+#pragma unroll
+      for (int g = 0; g < SP_G; ++g) w += inv[g] == 0.f ? 0.f : ex2(s[g] - top[g]) * inv[g];
+      if (k0 + u * THREADS < k_end && unsigned(page[u]) < unsigned(a.t.num_pages))
+        atomicAdd(a.key_mass + (size_t(page[u]) * a.t.P + off[u]) * a.HKV + kvh, w);
+    }
+  }
+}
+// the current token's own weight, stored where its row is
+__device__ __forceinline__ void add_new_weight(const SparseArgs& a, int b, int kvh, const float* s_new, const float* s_top,
+                                               const float* s_inv, float lifted) {
+  float w = 0.f;
+  for (int g = 0; g < a.G; ++g) w += ex2(s_new[g] - s_top[g]) * s_inv[g];
+  const int page = a.new_at[2 * b], off = a.new_at[2 * b + 1];
+  if (unsigned(page) < unsigned(a.t.num_pages) && unsigned(off) < unsigned(a.t.P))
+    a.key_mass[(size_t(page) * a.t.P + off) * a.HKV + kvh] = w * lifted;
+  else
+    atomicOr(a.t.status, DS_BAD_PAGE);
+}
+
+// The flat form's split: all steps of all (sequence, KV head) rows end to end, `per` of them to a CTA.  Whole warp.
+__device__ __forceinline__ int flat_steps(const SparseArgs& a, int b) {
+  return (seq_pages(a.t, b).ctx + SP_KEYS - 1) / SP_KEYS;
+}
+__device__ __forceinline__ int flat_per_cta(const SparseArgs& a) {
+  int total = 0;
+  for (int b = threadIdx.x & 31; b < a.t.B; b += 32) total += flat_steps(a, b);
+  total = __reduce_add_sync(0xffffffffu, total) * a.HKV;
+  return max(1, (total + a.n_cta - 1) / a.n_cta);
+}
+
+template <int D, int KVF, bool FLAT>
 __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KVF>::CTAS) sparse_decode_kernel(const SparseArgs a) {
   using C = SparseCfg<D, KVF>;
   constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS;
@@ -77,10 +139,31 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
   __shared__ float s_fac[16][SP_G], s_fin[2 * SP_G], s_new[SP_G];
   pdl_wait();
   pdl_launch();
-  cg::cluster_group cluster = cg::this_cluster();
-  const int NC = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
-  const int row = blockIdx.x / NC, b = row / a.HKV, kvh = row % a.HKV;
+  // the row of the grid that this CTA works on; in the flat form the first of them, and how many steps to do in all
+  int b, kvh, from = 0, todo = 0;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int NC = FLAT ? 1 : int(cluster.num_blocks()), rank = FLAT ? 0 : int(cluster.block_rank());
+  if constexpr (FLAT) {
+    __shared__ int s_flat[3];
+    if (warp == 0) {
+      const int per = flat_per_cta(a);
+      const int2 it = find_item(a.t.B, int(blockIdx.x) * per, [&](int i) { return flat_steps(a, i) * a.HKV; });
+      if (lane == 0) { s_flat[0] = per; s_flat[1] = it.x; s_flat[2] = it.y; }
+    }
+    __syncthreads();
+    todo = s_flat[0];
+    b = s_flat[1];
+    if (b < 0) return;  // more CTAs than steps
+    const int steps = flat_steps(a, b);
+    kvh = s_flat[2] / steps;
+    from = s_flat[2] % steps;
+  } else {
+    b = int(blockIdx.x) / NC / a.HKV;
+    kvh = int(blockIdx.x) / NC % a.HKV;
+  }
+  for (;;) {  // the flat form goes around once per row that it touches
+  const int row = b * a.HKV + kvh;
   const float scale_log2 = (a.sm_scale ? a.sm_scale[0] : rsqrtf(float(D))) * SP_LOG2E;
   // query fragments (B operand, heads on the n side).  bf16 / int8 cache: bf16 (int8: in the k order the byte-wise
   // fragments come out in).  E4M3: f16, after scaling each head by the power of two that brings its largest element to
@@ -156,7 +239,7 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
 
   // steps of 32 rows: this CTA's contiguous range, dealt to its warps in turn
   const int steps = (n_keys + SP_KEYS - 1) / SP_KEYS, per = (steps + NC - 1) / NC;
-  const int s_begin = min(steps, rank * per), s_end = min(steps, s_begin + per);
+  const int s_begin = FLAT ? from : min(steps, rank * per), s_end = min(steps, s_begin + (FLAT ? todo : per));
   const size_t row_stride = size_t(a.HKV) * C::ROWB;  // bytes between consecutive rows of a page plane
   // scores of this (sequence, KV head): behind S * P rows of every row of the grid, or behind the table entries before
   float* scores = a.scores;
@@ -453,7 +536,7 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
     o0[d1] = oacc[mt][2] * v_mul; o0[D + d1] = oacc[mt][3] * v_mul;
   }
   // the current token, taken from its own rows: one more partial (l = 1, o = v), merged by the cluster's first CTA
-  const bool has_new = a.k_new != nullptr && rank == 0;
+  const bool has_new = !FLAT && a.k_new != nullptr && rank == 0;  // (flat: in the second kernel)
   if (has_new) {
     const __nv_bfloat16* kp = a.k_new + size_t(row) * D;
     for (int g = warp; g < SP_G; g += WARPS) {
@@ -487,14 +570,28 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
     s_ml[SP_G + tid] = l;
   }
   __syncthreads();
+  // a row meets each CTA once and a CTA a row once, in the same order: row + CTA is a slot of their own
+  float* part = FLAT ? a.part_o + size_t(row + blockIdx.x) * (SP_G * D) : s_part;
   for (int i = tid; i < SP_G * D; i += THREADS) {
     const int g = i / D;
     float o = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) o += s_wo[w * SP_G * D + i] * s_fac[w][g];
     if (has_new) o += __bfloat162float(a.v_new[size_t(row) * D + i % D]) * s_fac[15][g];
-    s_part[i] = o;
+    part[i] = o;
   }
+  if constexpr (FLAT) {
+    if (tid < 2 * SP_G) a.part_ml[size_t(row + blockIdx.x) * (2 * SP_G) + tid] = s_ml[tid];
+    todo -= s_end - s_begin;
+    from = 0;
+    if (++kvh == a.HKV) {
+      kvh = 0;
+      do { ++b; } while (b < a.t.B && flat_steps(a, b) == 0);
+    }
+    if (todo <= 0 || b >= a.t.B) return;
+    __syncthreads();  // the ring and the partials' arrays are free
+    continue;
+  } else {
   cluster.sync();
   // every CTA finds the final maxima and sums and writes its share of the output
   __shared__ float s_cm[16][SP_G], s_cl[16][SP_G];
@@ -532,48 +629,97 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
         pack_bf16(o0 * inv, o1 * inv);
   }
   if (a.key_mass) {
-    // Four rows of every thread on their way together, no branch between them: rows behind the end read the last row's
-    // scores and add nothing.  (One warp per scheduler: what counts here is the number of instructions per row.)
-    constexpr int U = 4;
-    const int k_begin = s_begin * SP_KEYS, k_end = min(n_keys, s_end * SP_KEYS);
-    float top[SP_G], inv[SP_G];
-#pragma unroll
-    for (int g = 0; g < SP_G; ++g) {
-      top[g] = s_fin[g];
-      inv[g] = g < a.G ? s_fin[SP_G + g] * LIFTED : 0.f;
-    }
-    for (int k0 = k_begin + tid; k0 < k_end; k0 += U * THREADS) {
-      float4 lo[U], hi[U];
-      int page[U], off[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = min(k0 + u * THREADS, k_end - 1), e = a.t.page_of(k);
-        lo[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G);
-        hi[u] = *reinterpret_cast<const float4*>(scores + size_t(k) * SP_G + 4);
-        page[u] = a.t.indices[sp.first + (pages ? pages[e] : e)];  // no page: recorded by the step that read the row
-        off[u] = k - e * P;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float s[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
-        float w = 0.f;
-#pragma unroll
-        for (int g = 0; g < SP_G; ++g) w += inv[g] == 0.f ? 0.f : ex2(s[g] - top[g]) * inv[g];
-        if (k0 + u * THREADS < k_end && unsigned(page[u]) < unsigned(a.t.num_pages))
-          atomicAdd(a.key_mass + (size_t(page[u]) * P + off[u]) * a.HKV + kvh, w);
-      }
-    }
-    if (has_new && tid == 0) {
-      float w = 0.f;
-      for (int g = 0; g < a.G; ++g) w += ex2(s_new[g] - s_fin[g]) * s_fin[SP_G + g];
-      const int page = a.new_at[2 * b], off = a.new_at[2 * b + 1];
-      if (unsigned(page) < unsigned(a.t.num_pages) && unsigned(off) < unsigned(P))
-        a.key_mass[(size_t(page) * P + off) * a.HKV + kvh] = w * LIFTED;
-      else
-        atomicOr(a.t.status, DS_BAD_PAGE);
-    }
+    add_weights<THREADS>(a, sp, pages, kvh, scores, s_begin * SP_KEYS, min(n_keys, s_end * SP_KEYS), s_fin, s_fin + SP_G, LIFTED);
+    if (has_new && tid == 0) add_new_weight(a, b, kvh, s_new, s_fin, s_fin + SP_G, LIFTED);
   }
   cluster.sync();  // no CTA leaves while another still reads its shared memory
+  return;
+  }
+  }
+}
+
+// The flat form's second kernel: `chunks` CTAs per (sequence, KV head) merge its partials -- each a share of the output --
+// and turn a share of its scores into weights.
+template <int D, int KVF>
+__global__ void __launch_bounds__(256) sparse_merge_kernel(const SparseArgs a) {
+  constexpr float LIFTED = KVF == 1 ? 256.f : 1.f;
+  __shared__ int s_flat[2];
+  __shared__ float s_m[32][SP_G], s_l[32][SP_G], s_new[SP_G], s_top[SP_G], s_inv[SP_G];
+  extern __shared__ float s_fac[];  // [partials of the row][8]
+  pdl_wait();
+  pdl_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, b = row / a.HKV, kvh = row % a.HKV;
+  const SeqPages sp = seq_pages(a.t, b);
+  const int steps = flat_steps(a, b), P = a.t.P;
+  if (warp == 0) {
+    const int per = flat_per_cta(a);
+    int before = 0;
+    for (int i = lane; i < b; i += 32) before += flat_steps(a, i);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) { s_flat[0] = per; s_flat[1] = before * a.HKV + kvh * steps; }
+  }
+  if (a.k_new) {  // the current token, from its own rows: one more partial (l = 1, o = v)
+    const float scale_log2 = (a.sm_scale ? a.sm_scale[0] : rsqrtf(float(D))) * SP_LOG2E;
+    float dot = 0.f;
+    if (warp < a.G) {
+      const __nv_bfloat16 *kp = a.k_new + size_t(row) * D, *qp = a.q + (size_t(b) * a.HQ + size_t(kvh) * a.G + warp) * D;
+      for (int d = lane; d < D; d += 32) dot += __bfloat162float(qp[d]) * __bfloat162float(kp[d]);
+    }
+    dot = warp_sum(dot);
+    if (lane == 0) s_new[warp] = dot * scale_log2;
+  }
+  __syncthreads();
+  const int first = s_flat[1] / s_flat[0];
+  const int n = steps ? min(a.n_cta, (s_flat[1] + steps - 1) / s_flat[0] - first + 1) : 0;
+  const float* ml = a.part_ml + size_t(row + first) * (2 * SP_G);
+  {
+    const int g = tid % SP_G, j0 = tid / SP_G;
+    float m = -INFINITY, l = 0.f;
+    for (int j = j0; j < n; j += 32) m = fmaxf(m, ml[j * 2 * SP_G + g]);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int j = j0; j < n; j += 32) l += ml[j * 2 * SP_G + SP_G + g] * ex2(ml[j * 2 * SP_G + g] - base);
+    s_m[j0][g] = m;
+    s_l[j0][g] = l;
+  }
+  __syncthreads();
+  if (tid < SP_G) {
+    float m = a.k_new ? s_new[tid] : -INFINITY, l = 0.f;
+    for (int j = 0; j < 32; ++j) m = fmaxf(m, s_m[j][tid]);
+    const float base = m == -INFINITY ? 0.f : m;
+    for (int j = 0; j < 32; ++j) l += s_l[j][tid] * ex2(s_m[j][tid] - base);
+    if (a.k_new) l += ex2(s_new[tid] - base) * LIFTED;
+    s_top[tid] = base;
+    s_inv[tid] = l == 0.f ? 0.f : 1.f / l;
+  }
+  __syncthreads();
+  for (int i = tid; i < n * SP_G; i += 256) s_fac[i] = ex2(ml[i / SP_G * 2 * SP_G + i % SP_G] - s_top[i % SP_G]);
+  __syncthreads();
+  const int share = (SP_G * D / 2 + a.chunks - 1) / a.chunks;  // channel pairs per CTA
+  for (int i = chunk * share + tid; i < min(SP_G * D / 2, (chunk + 1) * share); i += 256) {
+    const int g = 2 * i / D, d = 2 * i % D;
+    if (g >= a.G) continue;
+    const float* po = a.part_o + size_t(row + first) * (SP_G * D) + 2 * i;
+    float o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float2 o = *reinterpret_cast<const float2*>(po + size_t(j) * (SP_G * D));
+      o0 += o.x * s_fac[j * SP_G + g];
+      o1 += o.y * s_fac[j * SP_G + g];
+    }
+    if (a.k_new) {
+      const float f = ex2(s_new[g] - s_top[g]) * LIFTED;
+      o0 += __bfloat162float(a.v_new[size_t(row) * D + d]) * f;
+      o1 += __bfloat162float(a.v_new[size_t(row) * D + d + 1]) * f;
+    }
+    const float inv = s_inv[g];
+    *reinterpret_cast<uint32_t*>(a.out + (size_t(b) * a.HQ + size_t(kvh) * a.G + g) * D + d) = pack_bf16(o0 * inv, o1 * inv);
+  }
+  if (!a.key_mass) return;
+  const float* scores = a.scores + (size_t(a.HKV) * sp.first + size_t(kvh) * sp.n) * size_t(P) * SP_G;
+  const int keys = (sp.ctx + a.chunks - 1) / a.chunks;
+  add_weights<256>(a, sp, nullptr, kvh, scores, chunk * keys, min(sp.ctx, (chunk + 1) * keys), s_top, s_inv, LIFTED);
+  if (a.k_new && chunk == 0 && tid == 0) add_new_weight(a, b, kvh, s_new, s_top, s_inv, LIFTED);
 }
 
 // CTAs per (sequence, KV head).  `slots` CTAs are resident at a time.
@@ -592,10 +738,19 @@ static int sparse_cluster(int64_t rows, int64_t steps, int slots, bool chosen) {
 template <int D, int KVF>
 static int launch_sparse(const SparseArgs& a, cudaStream_t stream) {
   using C = SparseCfg<D, KVF>;
-  const void* f = reinterpret_cast<const void*>(sparse_decode_kernel<D, KVF>);
+  const void* f = reinterpret_cast<const void*>(sparse_decode_kernel<D, KVF, false>);
   // the 48 KB that need no opt-in hold the static arrays too: head_dim 64 is above them with exactly 48 KB of ring
   Q35_TRY(ensure_dynamic_smem(f, C::SMEM > 49 * 1024 ? C::SMEM : 49 * 1024));
   const int64_t rows = int64_t(a.t.B) * a.HKV;
+  if (a.part_o) {
+    const void* flat = reinterpret_cast<const void*>(sparse_decode_kernel<D, KVF, true>);
+    Q35_TRY(ensure_dynamic_smem(flat, C::SMEM > 49 * 1024 ? C::SMEM : 49 * 1024));
+    launch_pdl(sparse_decode_kernel<D, KVF, true>, dim3(unsigned(a.n_cta)), dim3(32 * C::WARPS), C::SMEM, stream, a);
+    Q35_CUDA_LAUNCH_CHECK("attn.sparse_decode rows");
+    launch_pdl(sparse_merge_kernel<D, KVF>, dim3(unsigned(rows * a.chunks)), dim3(256), size_t(a.n_cta) * SP_G * 4, stream, a);
+    Q35_CUDA_LAUNCH_CHECK("attn.sparse_decode merge");
+    return 0;
+  }
   const int64_t keys = int64_t(a.t.P) * (a.pages ? a.S : (a.t.n_indices + a.t.B - 1) / a.t.B);
   const int cluster = sparse_cluster(rows, (keys + SP_KEYS - 1) / SP_KEYS, C::CTAS * sm_count(),
                                      a.pages != nullptr);
@@ -613,7 +768,7 @@ static int launch_sparse(const SparseArgs& a, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, sparse_decode_kernel<D, KVF>, a);
+    e = cudaLaunchKernelEx(&cfg, sparse_decode_kernel<D, KVF, false>, a);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();  // reported here, not by the caller's next CUDA call
@@ -659,7 +814,19 @@ int run_attn_sparse_decode(Call& c) {
   const int64_t S = pages.present ? pages.s[2] : 0;
   Q35_REQUIRE(S <= INT_MAX / P - 1 && B * HKV <= INT_MAX / 16, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
   const int64_t rows = pages.present ? B * HKV * S * P : HKV * int64_t(a.t.n_indices) * P;
-  Q35_TRY(c.workspace(mass.present ? rows * SP_G * 4 : 0, &ws));
+  // The flat form, for all pages of many rows: every CTA the same number of steps, whatever the lengths, a second kernel
+  // that merges.  It pays from 48 steps per CTA and 256 per row on (8 rows of 60000 bf16: 92 us, clusters 135; 74 rows of
+  // 32000 E4M3: 207 and 281; but 128 ragged rows of 73 steps: 85 and 72); below, and for chosen pages, whose rows are
+  // about equally long, one launch of clusters.
+  a.n_cta = sm_count() * (D == 256 ? (kv.fmt ? 2 : 1) : D == 128 ? (kv.fmt ? 3 : 2) : 4);
+  const int64_t all_steps = HKV * (int64_t(a.t.n_indices) * P / SP_KEYS);
+  const bool flat = !pages.present && all_steps >= 48 * int64_t(a.n_cta) && all_steps >= 256 * B * HKV;
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
+  const int64_t slots = flat ? B * HKV + a.n_cta : 0;
+  const int64_t o_scores = take(mass.present ? rows * SP_G * 4 : 0), o_po = take(slots * SP_G * D * 4),
+                o_ml = take(slots * 2 * SP_G * 4);
+  Q35_TRY(c.workspace(off, &ws));
   if (c.dry || B == 0) return 0;
   Q35_REQUIRE(aligned16(q.p) && aligned16(out.p), Q35_ERR_ALIGN, "%s: q and out must be 16-byte aligned", role);
   a.q = q.as<__nv_bfloat16>(); a.cache = static_cast<const uint8_t*>(kv.p);
@@ -671,7 +838,13 @@ int run_attn_sparse_decode(Call& c) {
   a.new_at = loc.present ? loc.as<int>() : nullptr;
   a.out = out.as<__nv_bfloat16>();
   a.key_mass = mass.present ? mass.as<float>() : nullptr;
-  a.scores = mass.present ? ws.as<float>() : nullptr;
+  a.scores = mass.present ? reinterpret_cast<float*>(ws.as<uint8_t>() + o_scores) : nullptr;
+  if (flat) {
+    a.part_o = reinterpret_cast<float*>(ws.as<uint8_t>() + o_po);
+    a.part_ml = reinterpret_cast<float*>(ws.as<uint8_t>() + o_ml);
+    const int64_t per_row = int64_t(a.t.n_indices) * P / B;  // the second kernel: a CTA per 2048 rows of the average one
+    a.chunks = int(per_row / 2048 + 1);
+  }
   a.HQ = int(HQ); a.HKV = int(HKV); a.G = int(HQ / HKV); a.S = int(S);
 #define Q35_SPARSE(DD)                                                 \
   (kv.fmt == 0 ? launch_sparse<DD, 0>(a, c.stream) : kv.fmt == 1 ? launch_sparse<DD, 1>(a, c.stream) \

@@ -233,6 +233,39 @@ def test_sparse_decode(fmt, D, HKV, G, P, S):
     assert q35.device_status() == 0
 
 
+@pytest.mark.parametrize("fmt,D,HKV,G,n", [("bf16", 256, 4, 2, 57344), ("int8", 128, 8, 3, 86016), ("e4m3c", 64, 16, 1, 57344)])
+def test_sparse_decode_of_many_rows_of_all_lengths(fmt, D, HKV, G, n):
+    """all pages of so many rows that every CTA gets an equal share of them, from none to half of them in one sequence"""
+    import ax_dsl_kernels_b200 as q35
+    ctxs, P = [0, 1, n // 2, 0, 33, n // 2 + 77, 0], 64
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 23, extra=10)
+    q = q_rows(len(ctxs), HKV * G, D, g, 2.0)
+    kn, vn = q_rows(len(ctxs), HKV, D, g), q_rows(len(ctxs), HKV, D, g)
+    spare = torch.arange(cache.shape[0], dtype=torch.int32)[~torch.isin(torch.arange(cache.shape[0]), table[1].long())]
+    loc = torch.stack([spare[:len(ctxs)], torch.arange(len(ctxs), dtype=torch.int32)], 1).contiguous()
+    old = torch.rand((cache.shape[0], P, HKV), generator=g)
+    need = q35.workspace_bytes("attn.sparse_decode", q=q, paged_kv_cache=cache, indptr=table[0], indices=table[1],
+                               last_page_len=table[2], out=q, **{{"row_scale": "paged_kv_scale"}.get(k, k): v for k, v in scales.items()})
+    assert need > 0  # the form with partial results in memory
+    ref, mass, size, reach = olc.sparse_decode(q, cache, *table, None, old, **scales, k_new=kn, v_new=vn, cache_location=loc)
+    gm = gpu(old)
+    args = (gpu(q), gpu(cache), *gpu(table))
+    kw = dict(k_new=gpu(kn), v_new=gpu(vn), **gpu_scales(scales))
+    out = q35.paged_attention_sparse(*args, key_mass=gm, cache_location=gpu(loc), **kw)
+    check_out(out, ref, size, reach, D, fmt)
+    check_mass(gm, mass, torch.zeros_like(old), reach.max(), D, n_add=8)
+    assert torch.equal(out, q35.paged_attention_sparse(*args, **kw))
+    # without the current token the empty sequences give zeros; the others agree with chosen pages that are all of them
+    out = q35.paged_attention_sparse(*args, **gpu_scales(scales))
+    every = torch.full((len(ctxs), HKV, max(-(-c // P) for c in ctxs)), -1, dtype=torch.int32)
+    for b, c in enumerate(ctxs):
+        every[b, :, :-(-c // P)] = torch.arange(-(-c // P), dtype=torch.int32)
+    other = q35.paged_attention_sparse(*args, gpu(every), **gpu_scales(scales))
+    assert (out[[0, 3, 6]] == 0).all()
+    assert ((out.float() - other.float()).abs() <= other.float().abs() * 2.0 ** -7 + 1e-5).all()
+    assert q35.device_status() == 0
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3c", "int8"])
 def test_sparse_decode_current_token(fmt):
     import ax_dsl_kernels_b200 as q35
