@@ -105,13 +105,13 @@ _ws_cache = {}  # (device index, stream) -> (bytes, address, tensor)
 
 
 def _workspace(dev, nbytes, stream):
-    """address of one growing scratch buffer per (device, stream), owned by the Python host (the library itself never
+    """(address, owner) of one growing scratch buffer per (device, stream), owned by the Python host (the library itself never
     allocates); roles running concurrently on different streams must not share scratch"""
     got = _ws_cache.get((dev, stream))
     if got is None or got[0] < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", dev))
         got = _ws_cache[dev, stream] = (buf.numel(), buf.data_ptr(), buf)
-    return got[1]
+    return got[1], got[2]
 
 
 def _scratch(dev, nbytes, stream):
@@ -121,7 +121,7 @@ def _scratch(dev, nbytes, stream):
     if torch.cuda.is_current_stream_capturing():
         own = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
         return own.data_ptr(), own
-    return _workspace(dev, nbytes, stream), None
+    return _workspace(dev, nbytes, stream)
 
 
 class _Plan:
@@ -169,8 +169,8 @@ def run_checked(role, stream=None, **tensors):
     if stream is None:
         stream = _raw_stream(dev)
     if plan.need:
-        own = _scratch(dev, plan.need, stream)
-        ptrs.append(own[0])
+        address, owner = _scratch(dev, plan.need, stream)  # owned until the call is issued: another thread may need more
+        ptrs.append(address)
     table = plan.words.from_buffer_copy(plan.bytes)
     i = _PTR_WORD
     for p in ptrs:

@@ -1,7 +1,8 @@
 // attn.evict: every (sequence, KV head) keeps the min(K, ctx) cached rows with the highest key_mass -- the first and the
 // last ones always, ties to the lower position -- and moves them, in order, to the sequence's first rows, in place.
 //
-// evict_choose, one CTA per (sequence, KV head): the weights once into registers as ordered integers, the border by block_kth, then one pass that writes the kept positions in ascending order.
+// evict_choose, one CTA per (sequence, KV head): the weights once into registers as ordered integers, the border by
+// block_kth, then one pass that writes the kept positions in ascending order.
 // evict_move: row j of the result is row kept[j] >= j of the cache.  Bound: HBM, every row that changes place read and
 // written once.
 //
@@ -10,8 +11,9 @@
 // only have to wait until the whole cluster has loaded that round.  A warp owns whole rows of a round: cp.async brings
 // them into its part of the shared memory, and it stores them from there while the cluster's barrier for the next round
 // closes and the one after that is on its way.  (An SM stores 27 bytes a cycle here; loads and barriers hide behind it.)
-// (32 x 4000 bf16 rows: one CTA per 64-byte column slice, without clusters, 121 us; one bulk copy per row and direction,
-// which the copy engine takes one in 16 ns, 66; this MOVE.)
+// (Choice and moves, 32 x 4000 of up to 16384 bf16 rows: one CTA per 64-byte column slice, without clusters, 175 us; this
+// 61.  115 MB read and written take 35 us at HBM's rate.  One bulk copy per row and direction instead of cp.async and
+// stores: as long.)
 #include <cooperative_groups.h>
 #include "abi.h"
 #include "attn_pages.cuh"

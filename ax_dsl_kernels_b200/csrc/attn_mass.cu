@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
     };
     if (SUM) load_keys(box_at(item), held, held_full);
     else load_block(item, held, held_full);
-    int y = SUM ? 0 : box_at(begin);
-    for (int t = 0; t < n; ++t) {
+    int y = SUM ? 0 : box_at(begin), t = 0;
+    for (; t < n; ++t) {
       const int s = t % C::STAGES, next = !SUM && t + 1 < n ? box_at(begin + t + 1) : -1;
       if (!mbar_wait(empty(s), (t / C::STAGES & 1) ^ 1)) {
         atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x10);
@@ -253,6 +253,9 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
       else load_keys(y, ring + s * C::OPERAND, full(s));
       y = next;
     }
+    // no load is on its way when the block ends, whichever wait ran out
+    mbar_wait(held_full, 0);
+    for (int k = max(0, t - C::STAGES); k < t; ++k) mbar_wait(full(k % C::STAGES), k / C::STAGES & 1);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
     if (elect_one()) {
@@ -261,7 +264,8 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
       // descriptors once: an offset in bytes / 16 is added to their address field (one thread issues all, instruction by
       // instruction: building a descriptor per MMA took longer than the MMA)
       const uint64_t held_desc = smem_desc(held, 16, 1024, 2), ring_desc = smem_desc(ring, 16, 1024, 2);
-      for (int t = 0; ok && t < n; ++t) {
+      int t = 0;
+      for (; ok && t < n; ++t) {
         const int s = t % C::STAGES, i = t % KM_ACC;
         if (!mbar_wait(acc_empty(i), (t / KM_ACC & 1) ^ 1)) {
           atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x20);
@@ -282,6 +286,8 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
         tc_commit(empty(s));
         tc_commit(acc_full(i));
       }
+      // nor a product
+      for (int k = max(0, t - KM_ACC); k < t; ++k) mbar_wait(acc_full(k % KM_ACC), k / KM_ACC & 1);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -439,7 +445,8 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
         const int e = a.t.page_of(key), page = page_at(a.t, sp.first + e);
         if (page >= 0) {
           float* dst = a.key_mass + (size_t(page) * a.t.P + (key - e * a.t.P)) * a.HKV + kvh;
-          *dst = a.accumulate ? *dst + total : total;
+          if (a.accumulate) atomicAdd(dst, total);  // a page may be listed by several sequences
+          else *dst = total;
         }
       }
     }

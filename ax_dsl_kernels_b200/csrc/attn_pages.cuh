@@ -132,12 +132,12 @@ inline int get_page_table(Call& c, const char* role, int64_t B, int64_t P, int64
   Q35_TRY(c.get("indices", M(Q35_I32), &indices));
   Q35_TRY(c.get("last_page_len", M(Q35_I32), &last));
   Q35_REQUIRE(indptr.numel() == B + 1 && last.numel() >= B, Q35_ERR_SHAPE, "%s: indptr [B + 1], last_page_len [B]", role);
-  Q35_REQUIRE(indices.numel() <= INT_MAX / P - 1, Q35_ERR_UNSUPPORTED,
-              "%s: %lld table entries of %lld rows: positions must fit 32 bits", role, (long long)indices.numel(),
+  Q35_REQUIRE(indices.numel() <= INT_MAX / 2 / P, Q35_ERR_UNSUPPORTED,  // kernels step behind the end before they look
+              "%s: %lld table entries of %lld rows: at most 2^30 positions", role, (long long)indices.numel(),
               (long long)P);
   t->indptr = indptr.as<int>(); t->indices = indices.as<int>(); t->last_page_len = last.as<int>();
   t->B = int(B); t->P = int(P); t->num_pages = int(num_pages); t->n_indices = int(indices.numel());
-  // n / P for n < 2^31: with 2^(l - 1) < P <= 2^l and m = floor(2^32 (2^l - P) / P) + 1, (umulhi(m, n) + n) >> l is exact
+  // n / P for n < 2^30: with 2^(l - 1) < P <= 2^l and m = floor(2^32 (2^l - P) / P) + 1, (umulhi(m, n) + n) >> l is exact
   int l = 0;
   while ((int64_t(1) << l) < P) ++l;
   t->p_mul = uint32_t((uint64_t(1) << 32) * ((uint64_t(1) << l) - uint64_t(P)) / uint64_t(P) + 1);

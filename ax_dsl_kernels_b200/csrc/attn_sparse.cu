@@ -7,7 +7,7 @@
 // Bound: HBM, K and V of the chosen rows once.  A cluster of C CTAs serves one (sequence, KV head): its chosen rows,
 // laid end to end, are cut into C contiguous ranges, every CTA runs one pass with a running maximum and sum over its
 // range, and the C partial results are merged through distributed shared memory -- one launch, no partials in HBM, no
-// counters.  Inside a CTA each warp takes steps of 32 rows through its own cp.async ring (16-byte chunks, XOR-swizzled
+// counters.  (All pages of many long rows: the flat form, equal shares per CTA and a second kernel that merges.)  Inside a CTA each warp takes steps of 32 rows through its own cp.async ring (16-byte chunks, XOR-swizzled
 // rows), with no block barrier in the loop.  Scores are computed transposed (S^T = K Q^T, mma.m16n8k16) so that the up
 // to 8 query heads of a KV head are the n = 8 side and O^T takes D / 4 registers a lane.
 //
@@ -812,7 +812,7 @@ int run_attn_sparse_decode(Call& c) {
   SparseArgs a{};
   Q35_TRY(get_page_table(c, role, B, P, kv.pages, &a.t));
   const int64_t S = pages.present ? pages.s[2] : 0;
-  Q35_REQUIRE(S <= INT_MAX / P - 1 && B * HKV <= INT_MAX / 16, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
+  Q35_REQUIRE(S <= INT_MAX / 2 / P && B * HKV <= INT_MAX / 16, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
   const int64_t rows = pages.present ? B * HKV * S * P : HKV * int64_t(a.t.n_indices) * P;
   // The flat form, for all pages of many rows: every CTA the same number of steps, whatever the lengths, a second kernel
   // that merges.  It pays from 48 steps per CTA and 256 per row on (8 rows of 60000 bf16: 92 us, clusters 135; 74 rows of
@@ -820,6 +820,7 @@ int run_attn_sparse_decode(Call& c) {
   // about equally long, one launch of clusters.
   a.n_cta = sm_count() * (D == 256 ? (kv.fmt ? 2 : 1) : D == 128 ? (kv.fmt ? 3 : 2) : 4);
   const int64_t all_steps = HKV * (int64_t(a.t.n_indices) * P / SP_KEYS);
+  Q35_REQUIRE(pages.present || all_steps + B * HKV <= INT_MAX, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
   const bool flat = !pages.present && all_steps >= 48 * int64_t(a.n_cta) && all_steps >= 256 * B * HKV;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };

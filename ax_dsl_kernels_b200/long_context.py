@@ -8,8 +8,9 @@
 
 All of them take the page table of paged_attention_decode: indptr [B + 1], indices, last_page_len [B] int32; sequence b
 has (pages - 1) * P + last_page_len[b] cached rows.  Rows and pages behind a sequence's end are neither read nor written.
-Pages that hold another sequence's rows too (a shared prefix) can be read by all of them; key_mass then adds up the
-weights of all their queries, and eviction, which moves rows, wants pages of its own.
+Pages that hold another sequence's rows too (a shared prefix) can be read by all of them.  Weights that are added to
+key_mass (paged_attention_sparse, paged_key_mass with accumulate) then add up over all their queries, in no fixed order;
+stored ones are those of one of the sequences; eviction, which moves rows, wants pages of its own.
 The reference has no counterpart of these operators; they extend its page-table form of decode attention
 (models/qwen35_35b_a3b/sgl/python/sgl_kernel_axera/attention/flash_attn.py:2549-2665)."""
 import torch
@@ -20,21 +21,24 @@ _keep = {}
 
 
 def _keep_pair(first, last, device):
-    """int32 [2] tensor (first, last) on `device`, made once per pair of values (a copy per call could not be captured
-    into a CUDA graph)"""
+    """int32 [2] tensor (first, last) on `device`, made once per pair of values; a pair first used inside a graph capture,
+    where nothing can be copied from the host, is set by the graph itself"""
     if first < 0 or last < 0:
         raise ValueError("keep_first and keep_last count pages or rows: not negative")
     key = (int(first), int(last), device.index)
     t = _keep.get(key)
-    if t is None:
+    if t is None and torch.cuda.is_current_stream_capturing():
+        t = torch.full((2,), int(first), dtype=torch.int32, device=device)
+        t[1:].fill_(int(last))
+    elif t is None:
         t = _keep[key] = torch.tensor([int(first), int(last)], dtype=torch.int32, device=device)
     return t
 
 
 def _scale(kw, sm_scale, device):
     if sm_scale is not None:
-        kw["sm_scale"] = sm_scale if isinstance(sm_scale, torch.Tensor) else torch.tensor(
-            [float(sm_scale)], dtype=torch.float32, device=device)
+        kw["sm_scale"] = sm_scale if isinstance(sm_scale, torch.Tensor) else torch.full(
+            (1,), float(sm_scale), dtype=torch.float32, device=device)
 
 
 def page_key_bounds(paged_kv_cache, indptr, indices, last_page_len, out=None, *, first_page=None, paged_kv_scale=None):
@@ -107,7 +111,8 @@ def paged_key_mass(q, paged_kv_cache, qo_indptr, indptr, indices, last_page_len,
     qo_indptr[b + 1] - qo_indptr[b] tokens of every sequence, whose K rows are in the cache already (the page table
     includes them, as in paged_attention_prefill); each sees the rows up to its own.  key_mass [pages, P, HKV] fp32: the
     sum over the window's queries and over the query heads of the KV head, stored for every row of every sequence
-    (accumulate: added).  Any number of query heads per KV head, any page size; head_dim 64, 128 or 256."""
+    (accumulate: added; the form for pages that several sequences list).  Up to 128 query heads per KV head, any page size;
+    head_dim 64, 128 or 256."""
     kw = dict(q=q, paged_kv_cache=paged_kv_cache, qo_indptr=qo_indptr, indptr=indptr, indices=indices,
               last_page_len=last_page_len, key_mass=key_mass)
     if accumulate:

@@ -368,6 +368,30 @@ def test_key_mass_weights_sum_to_the_number_of_query_rows(T):
         assert ((gm - gn).abs() <= gn * 2 * (2 * 260 * 2.0 ** -23 * float(reach.max()) + 2.0 ** -18) + 1e-30).all()
 
 
+def test_weights_of_shared_pages_add_up():
+    """eight sequences that share their first pages: every row gets the weight of all of them.  Eight terms in any order:
+    seven roundings of 2^-24 more than check_mass counts"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, n = 16, 2, 4, 128, 8
+    ctxs = [200 + 7 * i for i in range(n)]
+    cache, (indptr, indices, last), _, g = make(ctxs, P, HKV, D, "bf16", 31)
+    for b in range(1, n):  # the first ten pages are the first sequence's
+        indices[int(indptr[b]):int(indptr[b]) + 10] = indices[:10]
+    table = (indptr, indices, last)
+    T = [5 + b for b in range(n)]
+    q, qo = q_rows(sum(T), HKV * G, D, g, 2.0), torch.tensor([0, *torch.tensor(T).cumsum(0).tolist()], dtype=torch.int32)
+    old = torch.rand((cache.shape[0], P, HKV), generator=g)
+    ref, reach = olc.key_mass(q, cache, qo, *table, old, accumulate=True)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(qo), *gpu(table), gm, accumulate=True)
+    check_mass(gm, ref, torch.zeros_like(old), reach, D, n_add=sum(T) * G)
+    q1 = q_rows(n, HKV * G, D, g, 2.0)
+    _, ref, _, reach = olc.sparse_decode(q1, cache, *table, None, old)
+    gm = gpu(old)
+    q35.paged_attention_sparse(gpu(q1), gpu(cache), *gpu(table), key_mass=gm)
+    check_mass(gm, ref, torch.zeros_like(old), float(reach.max()), D, n_add=n * G)
+
+
 def test_key_mass_special_values():
     import ax_dsl_kernels_b200 as q35
     P, HKV, G, D = 16, 1, 4, 64
@@ -547,6 +571,33 @@ def test_captured_and_replayed_and_on_another_stream():
         graphs[i].replay()
         assert all(torch.equal(a, b) for a, b in zip(state(), want[i]))
     assert q35.device_status() == 0
+
+
+def test_first_calls_inside_a_capture():
+    """counts and scales that no call has used yet: nothing is copied from the host"""
+    import ax_dsl_kernels_b200 as q35
+    cache, table, _, g = make([700, 300], 16, 2, 128, "bf16", 23)
+    gt, gc, q = gpu(table), gpu(cache), gpu(q_rows(2, 16, 128, g))
+    bounds, qo = q35.page_key_bounds(gc, *gt), gpu(torch.tensor([0, 1, 2], dtype=torch.int32))
+
+    def step(first, last, scale):
+        pages = q35.select_pages(q, bounds, *gt, 9, keep_first=first, keep_last=last)
+        gm = torch.zeros((cache.shape[0], 16, 2), device="cuda")
+        out = q35.paged_attention_sparse(q, gc, *gt, pages, key_mass=gm, sm_scale=scale)
+        q35.paged_key_mass(q, gc, qo, *gt, gm, accumulate=True, sm_scale=scale)
+        return pages, out, gm
+
+    step(0, 1, None)  # the library itself is loaded
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(6, 2, 0.0625)
+    graph.replay()
+    assert not any(k[:2] == (6, 2) for k in q35.long_context._keep)
+    for a, b in zip(got, step(6, 2, 0.0625)):
+        assert torch.equal(a, b)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], step(6, 2, 0.0625)[0]) and q35.device_status() == 0
 
 
 def test_a_captured_graph_keeps_its_own_scratch():

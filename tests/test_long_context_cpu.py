@@ -56,6 +56,18 @@ def test_scratch_of_an_eviction_from_a_long_table():
     assert _lib.workspace_bytes("attn.evict", **t) == 5000 * P * HKV * 4
 
 
+@pytest.mark.parametrize("role", sorted(r for r in ROLES if r != "attn.select_pages"))
+def test_tables_of_more_than_2_30_positions_are_refused(role):
+    for n, ok in ((2 ** 30 // P - 1, True), (2 ** 30 // P, False)):
+        t = dict(ROLES[role], indices=torch.empty(n, dtype=i32, device="meta"))
+        if ok:
+            assert _lib.workspace_bytes(role, **t) >= 0
+            continue
+        with pytest.raises(_lib.Q35Error) as e:
+            _lib.workspace_bytes(role, **t)
+        assert e.value.status == UNSUPPORTED
+
+
 def test_scratch_of_the_weights():
     with_mass = dict(ROLES["attn.sparse_decode"], key_mass=MASS)
     assert _lib.workspace_bytes("attn.sparse_decode", **with_mass) == HKV * N * P * 32
