@@ -34,6 +34,7 @@ struct EvictArgs {
   int HKV, K, row_bytes;       // row_bytes of one head
   int cap;                     // rows whose keys fit the shared memory
   int per_warp;                // rows per warp and round of moves
+  int planes;                  // of a row per CTA: 2 = K and V, 1 = one of them (blockIdx.y)
 };
 
 constexpr int EV_THREADS = 1024;
@@ -233,20 +234,21 @@ __global__ void __launch_bounds__(EM_THREADS, 1) evict_move_kernel(const EvictAr
       atomicOr(a.t.status, DS_BAD_PAGE);
     }
   };
-  // 16-byte pieces, pp to a row (K, then V): a lane's PL pieces of every row that it takes part in, `rows` rows to an
+  // 16-byte pieces, pp to a row (K, then V, or one of them): a lane's PL pieces of every row that it takes part in, `rows` rows to an
   // instruction of the warp where a row has fewer than 32
-  const int pr = a.row_bytes / 16, pp = 2 * pr, rows = pp < 32 ? 32 / pp : 1;
+  const int pr = a.row_bytes / 16, pp = a.planes * pr, rows = pp < 32 ? 32 / pp : 1;
   const int sub = pp < 32 ? lane / pp : 0, piece0 = pp < 32 ? lane % pp : lane;
-  const int64_t v_off = v_rows * a.row_bytes;
+  const int64_t v_off = v_rows * a.row_bytes, own_off = blockIdx.y ? v_off : 0;
+  const bool has_k = blockIdx.y == 0, has_v = a.planes == 2 || blockIdx.y == 1;
   int64_t in_cache[PL];
   bool has[PL];
 #pragma unroll
   for (int q = 0; q < PL; ++q) {
     const int p = piece0 + 32 * q;
     has[q] = sub < rows && p < pp;
-    in_cache[q] = p < pr ? p * 16 : v_off + (p - pr) * 16;
+    in_cache[q] = p < pr ? own_off + p * 16 : v_off + (p - pr) * 16;
   }
-  uint8_t* const ring = smem + size_t(warp) * RW * 2 * a.row_bytes;  // the warp's rows in buffer 0
+  uint8_t* const ring = smem + size_t(warp) * RW * a.planes * a.row_bytes;  // the warp's rows in buffer 0
   auto pieces = [&](int64_t where, auto f) {  // f(address in the cache, offset in the warp's buffer) for every piece
     const unsigned long long mine = where >= 0 ? reinterpret_cast<unsigned long long>(a.cache) + where * a.row_bytes : 0ull;
 #pragma unroll 4
@@ -266,10 +268,10 @@ __global__ void __launch_bounds__(EM_THREADS, 1) evict_move_kernel(const EvictAr
     pieces(from[u], [&](uint8_t* src, int off) { cp_async_16(base + off, src); });
     cp_async_commit();
     if (from[u] >= 0) {
-      mass[u] = *mass_at(from[u]);
+      if (has_k) mass[u] = *mass_at(from[u]);
       if (a.row_scale) {
-        ks[u] = a.row_scale[from[u]];
-        vs[u] = a.row_scale[from[u] + v_rows];
+        if (has_k) ks[u] = a.row_scale[from[u]];
+        if (has_v) vs[u] = a.row_scale[from[u] + v_rows];
       }
     }
     pos_cur = pos_next;
@@ -282,10 +284,10 @@ __global__ void __launch_bounds__(EM_THREADS, 1) evict_move_kernel(const EvictAr
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(base + off);
     });
     if (to[u] >= 0) {
-      *mass_at(to[u]) = mass[u];
+      if (has_k) *mass_at(to[u]) = mass[u];
       if (a.row_scale) {
-        a.row_scale[to[u]] = ks[u];
-        a.row_scale[to[u] + v_rows] = vs[u];
+        if (has_k) a.row_scale[to[u]] = ks[u];
+        if (has_v) a.row_scale[to[u] + v_rows] = vs[u];
       }
     }
   };
@@ -321,7 +323,7 @@ static int launch_evict_move(const EvictArgs& a, int rows, int cluster, cudaStre
   if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(rows * cluster));
+    cfg.gridDim = dim3(unsigned(rows * cluster), unsigned(2 / a.planes));
     cfg.blockDim = dim3(EM_THREADS);
     cfg.dynamicSmemBytes = 3 * EM_BUF;
     cfg.stream = stream;
@@ -378,13 +380,21 @@ int run_attn_evict(Call& c) {
   launch_pdl(evict_choose_kernel, dim3(unsigned(rows)), dim3(EV_THREADS),
              positions > EV_REGS * EV_THREADS ? size_t(a.cap) * 4 : 0, c.stream, a);
   Q35_CUDA_LAUNCH_CHECK("attn.evict choice");
-  // as many CTAs per (sequence, KV head) as run at once on an SM each, while a round gives every one of them rows
-  a.per_warp = EM_BUF / (2 * a.row_bytes * EM_WARPS) < 32 ? EM_BUF / (2 * a.row_bytes * EM_WARPS) : 32;
+  // as many CTAs per (sequence, KV head) as run at once on an SM each, while a round gives every one of them rows; K and
+  // V, which are moved alike, each by a cluster of its own where the SMs are enough for both
+  auto per_warp = [&](int planes) {
+    const int n = EM_BUF / (planes * a.row_bytes * EM_WARPS);
+    return n < 32 ? n : 32;
+  };
+  a.planes = 2;
   int cluster = 1;
-  while (cluster < 16 && rows * cluster * 2 <= sm_count() && int64_t(cluster) * a.per_warp * EM_WARPS < a.K) cluster *= 2;
-  Q35_TRY(a.row_bytes <= 256   ? launch_evict_move<1>(a, int(rows), cluster, c.stream)
-          : a.row_bytes <= 512 ? launch_evict_move<2>(a, int(rows), cluster, c.stream)
-                               : launch_evict_move<EM_PIECES>(a, int(rows), cluster, c.stream));
+  while (cluster < 16 && rows * cluster * 2 <= sm_count() && int64_t(cluster) * per_warp(2) * EM_WARPS < a.K) cluster *= 2;
+  if (rows * cluster * 2 <= sm_count() && int64_t(cluster) * per_warp(1) * EM_WARPS < a.K) a.planes = 1;
+  a.per_warp = per_warp(a.planes);
+  const int bytes = a.planes * a.row_bytes;
+  Q35_TRY(bytes <= 512    ? launch_evict_move<1>(a, int(rows), cluster, c.stream)
+          : bytes <= 1024 ? launch_evict_move<2>(a, int(rows), cluster, c.stream)
+                          : launch_evict_move<EM_PIECES>(a, int(rows), cluster, c.stream));
   return 0;
 }
 
