@@ -1,7 +1,7 @@
 // attn.evict: every (sequence, KV head) keeps the min(K, ctx) cached rows with the highest key_mass -- the first and the
 // last ones always, ties to the lower position -- and moves them, in order, to the sequence's first rows, in place.
 //
-// evict_choose, one CTA per (sequence, KV head): the weights once into registers as ordered integers, the border by
+// evict_choose, a cluster per (sequence, KV head): the weights once into registers as ordered integers, the border by
 // block_kth, then one pass that writes the kept positions in ascending order.
 // evict_move: row j of the result is row kept[j] >= j of the cache.  Bound: HBM, every row that changes place read and
 // written once.
@@ -32,56 +32,64 @@ struct EvictArgs {
   int* kept;                   // [B, HKV, K]
   uint32_t* keys;              // workspace [HKV * n_indices * P], for rows that do not fit the shared memory
   int HKV, K, row_bytes;       // row_bytes of one head
-  int cap;                     // rows whose keys fit the shared memory
+  int cap;                     // rows whose keys fit a CTA's shared memory
   int per_warp;                // rows per warp and round of moves
   int planes;                  // of a row per CTA: 2 = K and V, 1 = one of them (blockIdx.y)
 };
 
 constexpr int EV_THREADS = 1024;
-constexpr int EV_REGS = 16;         // keys per thread in registers: sequences of up to 16384 rows
+constexpr int EV_REGS = 16;         // most keys per thread in registers: 16384 rows per CTA
 constexpr int EV_CAP = 48 * 1024;   // keys in shared memory, 192 KB, where the registers do not hold them
-constexpr int EV_U = 8;             // positions per thread and round
+constexpr int EV_U = 8;             // most positions per thread and round
 
 struct ChooseScratch {
   KthScratch<EV_THREADS> kth;
   int count[2][EV_U][32], gt[32], eq[32];
+  int sums[2];  // rows above the border and rows equal to it, read by the cluster
 };
 
-// The choice for one (sequence, KV head) of n > K rows.  Thread t looks at the positions t, t + 1024, ...; key(m) is the
-// key of position m * 1024 + t, set by put(m, key).  M: static number of keys per thread (0: n / 1024, in a loop).
+// The choice for one (sequence, KV head) of n > K rows, by a cluster: every CTA takes a range of positions, whose keys it
+// holds -- key(m) is that of position p0 + m * 1024 + t, set by put(m, key) -- and writes the kept ones among them.
+// M: static number of keys per thread (0: as many as there are, in a loop).
 template <int M, typename Put, typename Key>
-__device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages& sp, int h, int* out, ChooseScratch& s,
-                                             Put put, Key key) {
+__device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages& sp, int h, int p0, int p1, int* out,
+                                             ChooseScratch& s, Put put, Key key) {
+  constexpr int U = M && M < EV_U ? M : EV_U;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int NC = int(cluster.num_blocks()), crank = int(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = sp.ctx, K = a.K, P = a.t.P;
   const int last = a.keep ? min(max(a.keep[1], 0), K) : 0;
   const int first = a.keep ? min(max(a.keep[0], 0), K - last) : 0;
   const int rank = K - first - last, f0 = first, f1 = n - last;  // the free rows, of which `rank` are kept
-  const int rounds = M ? M : (n + EV_THREADS - 1) / EV_THREADS;
+  const int rounds = M ? M : (p1 - p0 + EV_THREADS - 1) / EV_THREADS;
+  auto position = [&](int m) { return p0 + m * EV_THREADS + tid; };
   auto is_free = [&](int m) {
-    const int i = m * EV_THREADS + tid;
-    return i >= f0 && i < f1;
+    const int i = position(m);
+    return i >= f0 && i < f1 && i < p1;
   };
   uint32_t border = 0u;
   int equal = 0;         // how many of the rows that equal the border are kept
   bool ties = false;     // and whether that is not all of them
+  int seen = 0;          // rows equal to the border before this round of positions
+  int done = min(p0, f0) + max(0, p0 - f1);  // and kept rows
   if (rank > 0) {
     bool bad = false;
 #pragma unroll
-    for (int m0 = 0; m0 < rounds; m0 += EV_U) {
-      int page[EV_U], off[EV_U];
+    for (int m0 = 0; m0 < rounds; m0 += U) {
+      int page[U], off[U];
 #pragma unroll
-      for (int u = 0; u < EV_U; ++u) {
-        const int i = min((m0 + u) * EV_THREADS + tid, n - 1), e = a.t.page_of(i);
+      for (int u = 0; u < U; ++u) {
+        const int i = min(position(m0 + u), n - 1), e = a.t.page_of(i);
         page[u] = page_or_first(a.t, sp.first + e, bad);
         off[u] = i - e * P;
       }
-      float w[EV_U];
+      float w[U];
 #pragma unroll
-      for (int u = 0; u < EV_U; ++u) w[u] = a.key_mass[(size_t(page[u]) * P + off[u]) * a.HKV + h];
+      for (int u = 0; u < U; ++u) w[u] = a.key_mass[(size_t(page[u]) * P + off[u]) * a.HKV + h];
 #pragma unroll
-      for (int u = 0; u < EV_U; ++u)
-        if (M || (m0 + u) * EV_THREADS + tid < n) put(m0 + u, order_key(w[u]));
+      for (int u = 0; u < U; ++u)
+        if (M || position(m0 + u) < p1) put(m0 + u, order_key(w[u]));
     }
     if (bad) atomicOr(a.t.status, DS_BAD_PAGE);
     auto each = [&](auto f) {
@@ -89,7 +97,7 @@ __device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages&
       for (int m = 0; m < rounds; ++m)
         if (is_free(m)) f(key(m));
     };
-    border = block_kth<EV_THREADS, false>(each, rank, s.kth);
+    border = block_kth<EV_THREADS, false, true>(each, rank, s.kth);
     int gt = 0, eq = 0;
     each([&](uint32_t k) {
       gt += k > border;
@@ -99,58 +107,68 @@ __device__ __forceinline__ void evict_choose(const EvictArgs& a, const SeqPages&
     eq = __reduce_add_sync(0xffffffffu, eq);
     if (lane == 0) { s.gt[warp] = gt; s.eq[warp] = eq; }
     __syncthreads();
-    equal = rank - __reduce_add_sync(0xffffffffu, s.gt[lane]);
-    ties = equal != __reduce_add_sync(0xffffffffu, s.eq[lane]);
+    gt = __reduce_add_sync(0xffffffffu, s.gt[lane]);
+    eq = __reduce_add_sync(0xffffffffu, s.eq[lane]);
+    if (tid == 0) { s.sums[0] = gt; s.sums[1] = eq; }
+    cluster.sync();
+    const int* sums = cluster.map_shared_rank(s.sums, lane % NC);
+    gt = lane < NC ? sums[0] : 0;
+    eq = lane < NC ? sums[1] : 0;
+    equal = rank - __reduce_add_sync(0xffffffffu, gt);
+    ties = equal != __reduce_add_sync(0xffffffffu, eq);
+    seen = __reduce_add_sync(0xffffffffu, lane < crank ? eq : 0);
+    done += __reduce_add_sync(0xffffffffu, lane < crank ? gt : 0) + min(seen, equal);
   }
+  auto gathered = cluster.barrier_arrive();  // nobody reads another's scratch from here on
   // how many flags are set before each of the thread's positions of a round; returns how many in all.  Calls alternate
   // between two sets of counts: one barrier each.
   int turn = 0;
-  auto scan = [&](const bool (&flag)[EV_U], int (&at)[EV_U]) {
+  auto scan = [&](const bool (&flag)[U], int (&at)[U]) {
     int (&count)[EV_U][32] = s.count[turn ^= 1];
-    unsigned ball[EV_U];
+    unsigned ball[U];
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       ball[u] = __ballot_sync(0xffffffffu, flag[u]);
       if (lane == 0) count[u][warp] = __popc(ball[u]);
     }
     __syncthreads();
     int total = 0;
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int c = count[u][lane];
       at[u] = total + __reduce_add_sync(0xffffffffu, lane < warp ? c : 0) + __popc(ball[u] & ((1u << lane) - 1));
       total += __reduce_add_sync(0xffffffffu, c);
     }
     return total;
   };
-  int done = 0, seen = 0;  // kept rows, and rows equal to the border, before this round of positions
 #pragma unroll
-  for (int m0 = 0; m0 < rounds; m0 += EV_U) {
-    if (m0 * EV_THREADS >= n) break;
-    bool take[EV_U], eq[EV_U];
-    int at[EV_U];
+  for (int m0 = 0; m0 < rounds; m0 += U) {
+    if (p0 + m0 * EV_THREADS >= p1) break;
+    bool take[U], eq[U];
+    int at[U];
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u) {
-      const int m = m0 + u, i = m * EV_THREADS + tid;
+    for (int u = 0; u < U; ++u) {
+      const int m = m0 + u, i = position(m);
       const bool free_row = is_free(m) && rank > 0;
       const uint32_t k = free_row ? key(m) : 0u;
       eq[u] = free_row && k == border;
-      take[u] = i < n && (i < f0 || i >= f1 || (free_row && k > border));
+      take[u] = i < p1 && (i < f0 || i >= f1 || (free_row && k > border));
     }
     if (ties) {
       const int total = scan(eq, at);
 #pragma unroll
-      for (int u = 0; u < EV_U; ++u) eq[u] = eq[u] && seen + at[u] < equal;
+      for (int u = 0; u < U; ++u) eq[u] = eq[u] && seen + at[u] < equal;
       seen += total;
     }
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u) take[u] |= eq[u];
+    for (int u = 0; u < U; ++u) take[u] |= eq[u];
     const int total = scan(take, at);
 #pragma unroll
-    for (int u = 0; u < EV_U; ++u)
-      if (take[u] && done + at[u] < K) out[done + at[u]] = (m0 + u) * EV_THREADS + tid;
+    for (int u = 0; u < U; ++u)
+      if (take[u] && done + at[u] < K) out[done + at[u]] = position(m0 + u);
     done += total;
   }
+  cluster.barrier_wait(std::move(gathered));
 }
 
 __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArgs a) {
@@ -158,22 +176,28 @@ __global__ void __launch_bounds__(EV_THREADS) evict_choose_kernel(const EvictArg
   __shared__ ChooseScratch s;
   pdl_wait();
   pdl_launch();
-  const int tid = threadIdx.x, b = blockIdx.x / a.HKV, h = blockIdx.x % a.HKV;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int NC = int(cluster.num_blocks()), crank = int(cluster.block_rank());
+  const int tid = threadIdx.x, row = blockIdx.x / NC, b = row / a.HKV, h = row % a.HKV;
   const SeqPages sp = seq_pages(a.t, b);
-  int* out = a.kept + size_t(blockIdx.x) * a.K;
-  if (sp.ctx <= a.K) {
-    for (int i = tid; i < a.K; i += EV_THREADS) out[i] = i < sp.ctx ? i : -1;
+  int* out = a.kept + size_t(row) * a.K;
+  if (sp.ctx <= a.K) {  // the whole cluster
+    for (int i = crank * EV_THREADS + tid; i < a.K; i += NC * EV_THREADS) out[i] = i < sp.ctx ? i : -1;
     return;
   }
-  if (sp.ctx <= EV_REGS / 2 * EV_THREADS) {
-    uint32_t k[EV_REGS / 2];
-    evict_choose<EV_REGS / 2>(a, sp, h, out, s, [&](int m, uint32_t x) { k[m] = x; }, [&](int m) { return k[m]; });
-  } else if (sp.ctx <= EV_REGS * EV_THREADS) {
-    uint32_t k[EV_REGS];
-    evict_choose<EV_REGS>(a, sp, h, out, s, [&](int m, uint32_t x) { k[m] = x; }, [&](int m) { return k[m]; });
-  } else {
-    uint32_t* keys = sp.ctx <= a.cap ? s_keys : a.keys + (size_t(a.HKV) * sp.first + size_t(h) * sp.n) * a.t.P;
-    evict_choose<0>(a, sp, h, out, s, [&](int m, uint32_t x) { keys[m * EV_THREADS + tid] = x; },
+  const int part = (sp.ctx + NC - 1) / NC, p0 = min(sp.ctx, crank * part), p1 = min(sp.ctx, p0 + part);
+  auto in_registers = [&](auto m) {
+    uint32_t k[decltype(m)::value];
+    evict_choose<decltype(m)::value>(a, sp, h, p0, p1, out, s, [&](int i, uint32_t x) { k[i] = x; },
+                                     [&](int i) { return k[i]; });
+  };
+  if (part <= 2 * EV_THREADS) in_registers(std::integral_constant<int, 2>());
+  else if (part <= 4 * EV_THREADS) in_registers(std::integral_constant<int, 4>());
+  else if (part <= 8 * EV_THREADS) in_registers(std::integral_constant<int, 8>());
+  else if (part <= EV_REGS * EV_THREADS) in_registers(std::integral_constant<int, EV_REGS>());
+  else {
+    uint32_t* keys = part <= a.cap ? s_keys : a.keys + (size_t(a.HKV) * sp.first + size_t(h) * sp.n) * a.t.P + p0;
+    evict_choose<0>(a, sp, h, p0, p1, out, s, [&](int m, uint32_t x) { keys[m * EV_THREADS + tid] = x; },
                     [&](int m) { return keys[m * EV_THREADS + tid]; });
   }
 }
@@ -315,17 +339,15 @@ __global__ void __launch_bounds__(EM_THREADS, 1) evict_move_kernel(const EvictAr
   }
 }
 
-template <int PL>
-static int launch_evict_move(const EvictArgs& a, int rows, int cluster, cudaStream_t stream) {
-  const void* f = reinterpret_cast<const void*>(evict_move_kernel<PL>);
-  Q35_TRY(ensure_dynamic_smem(f, 3 * EM_BUF));
+template <typename F>
+static int launch_evict(F f, const EvictArgs& a, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (cluster > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (cluster > 8) e = cudaFuncSetAttribute(reinterpret_cast<const void*>(f), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(rows * cluster), unsigned(2 / a.planes));
-    cfg.blockDim = dim3(EM_THREADS);
-    cfg.dynamicSmemBytes = 3 * EM_BUF;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -333,14 +355,21 @@ static int launch_evict_move(const EvictArgs& a, int rows, int cluster, cudaStre
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, evict_move_kernel<PL>, a);
+    e = cudaLaunchKernelEx(&cfg, f, a);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();  // reported here, not by the caller's next CUDA call
     return fail(Q35_ERR_CUDA, "attn.evict: %s", cudaGetErrorString(e));
   }
-  Q35_CUDA_LAUNCH_CHECK("attn.evict moves");
+  Q35_CUDA_LAUNCH_CHECK("attn.evict");
   return 0;
+}
+
+template <int PL>
+static int launch_evict_move(const EvictArgs& a, int rows, int cluster, cudaStream_t stream) {
+  Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(evict_move_kernel<PL>), 3 * EM_BUF));
+  return launch_evict(evict_move_kernel<PL>, a, dim3(unsigned(rows * cluster), unsigned(2 / a.planes)), EM_THREADS,
+                      3 * EM_BUF, cluster, stream);
 }
 
 int run_attn_evict(Call& c) {
@@ -376,10 +405,12 @@ int run_attn_evict(Call& c) {
   a.keys = ws.present ? ws.as<uint32_t>() : nullptr;
   const int64_t rows = B * kv.HKV;
   Q35_TRY(ensure_dynamic_smem(reinterpret_cast<const void*>(evict_choose_kernel), EV_CAP * 4));
+  // as many CTAs per (sequence, KV head) as there are SMs for and rows of the average sequence to give each two a thread
+  int choosers = 1;
+  while (choosers < 8 && rows * choosers * 2 <= sm_count() && positions > B * choosers * 2 * EV_THREADS) choosers *= 2;
   // (no keys in shared memory where every sequence fits the registers)
-  launch_pdl(evict_choose_kernel, dim3(unsigned(rows)), dim3(EV_THREADS),
-             positions > EV_REGS * EV_THREADS ? size_t(a.cap) * 4 : 0, c.stream, a);
-  Q35_CUDA_LAUNCH_CHECK("attn.evict choice");
+  Q35_TRY(launch_evict(evict_choose_kernel, a, dim3(unsigned(rows * choosers)), EV_THREADS,
+                       positions > int64_t(choosers) * EV_REGS * EV_THREADS ? size_t(a.cap) * 4 : 0, choosers, c.stream));
   // as many CTAs per (sequence, KV head) as run at once on an SM each, while a round gives every one of them rows; K and
   // V, which are moved alike, each by a cluster of its own where the SMs are enough for both
   auto per_warp = [&](int planes) {

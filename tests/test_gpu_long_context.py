@@ -447,6 +447,23 @@ def test_evict_from_more_rows_than_fit_on_chip():
     assert q35.device_status() == 0
 
 
+@pytest.mark.parametrize("n,long,K", [(76, 60001, 40000), (76, 20000, 1500), (40, 60001, 900), (40, 130000, 100000), (16, 9000, 333)])
+def test_evict_of_many_rows_of_all_lengths(n, long, K):
+    """one, two and four blocks to a row's choice: keys in registers, in shared memory, in scratch memory; equal weights
+    across the blocks' borders"""
+    import ax_dsl_kernels_b200 as q35
+    ctxs = [long] + [(97 * i) % 2000 for i in range(n - 1)]
+    cache, table, scales, g = make(ctxs, 64, 1, 64, "int8", 24)
+    for mass in (torch.randn((cache.shape[0], 64, 1), generator=g).mul(2).exp(),
+                 torch.randint(0, 5, (cache.shape[0], 64, 1), generator=g).float()):
+        ref, rcache, rmass, rrs = olc.evict(cache, mass, *table, K, 3, 60, scales["row_scale"])
+        gc, gm, gs = gpu(cache), gpu(mass), gpu_scales(scales)
+        kept = q35.evict_keys(gc, gm, *gpu(table), K, keep_first=3, keep_last=60, **gs)
+        assert torch.equal(kept.cpu(), ref)
+        assert torch.equal(gc.cpu(), rcache) and torch.equal(gm.cpu(), rmass) and torch.equal(gs["paged_kv_scale"].cpu(), rrs)
+    assert q35.device_status() == 0
+
+
 @pytest.mark.parametrize("ctx,K", [(5000, 4096), (9000, 1100)])
 def test_evict_ties_and_special_values(ctx, K):
     import ax_dsl_kernels_b200 as q35
