@@ -9,7 +9,7 @@
 // Bound, for long windows: the tensor pipe and the special-function unit alike (a 128 x 128 tile of D = 256 is 1024
 // cycles of MMA and 1024 of exponentials), for short ones the launches and one tile's latency.
 //
-// Both passes are the same pipeline, one CTA per item: a warp of TMA loads, a warp that issues tcgen05.mma (M = N = 128,
+// Both passes are the same pipeline: a warp of TMA loads, a warp that issues tcgen05.mma (M = N = 128,
 // fp32 accumulators in tensor memory, four of them), and four groups of four warps that read one each in turn.
 // Pass 1 holds a block of query rows (lanes) and streams 128-key tiles (columns): a thread owns a query row and keeps
 // its running maximum and sum.  Pass 2 holds a 128-key tile (lanes) and streams the blocks of query rows that see it: a
@@ -36,6 +36,7 @@ constexpr int KM_GROUPS = 4;    // groups of four warps that read accumulators
 constexpr int KM_THREADS = 128 + 128 * KM_GROUPS;  // TMA, MMA, two spare warps, the groups
 constexpr int KM_ACC = KM_GROUPS;  // accumulators of 128 columns, all of tensor memory.  A group always reads the same one:
                                 // it waits for the next phase of that one's barrier and cannot take an older for it
+constexpr int KM_ITEMS = 16;    // most tiles of a CTA in pass 2
 constexpr float KM_LOG2E = 1.4426950408889634f;
 
 struct MassArgs {
@@ -134,18 +135,27 @@ struct MassCfg {
   static constexpr int SMEM = 1024 + (1 + STAGES) * OPERAND;
 };
 
+// What a CTA works on: a block of query rows (pass 1) or a tile of keys (pass 2) of one (sequence, KV head), and the n
+// tiles or blocks from `begin` on that it meets; the first of them is the CTA's t0-th.
+struct MassItem {
+  int b, index, kvh, begin, n, t0;
+  SeqPages sp;
+  Window w;
+  float scale;
+};
+
 template <int D, bool SUM>
 __global__ void __launch_bounds__(KM_THREADS, 1)
     mass_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const MassArgs a) {
   using C = MassCfg<D>;
   using namespace tc;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * C::STAGES + 2 * KM_ACC + 1];
+  __shared__ __align__(8) uint64_t s_bar[2 * C::STAGES + 2 * KM_ACC + 2];
   __shared__ uint32_t s_tmem;
-  __shared__ int2 s_item;
+  __shared__ MassItem s_item[KM_ITEMS];
   __shared__ __align__(16) float s_lse[KM_GROUPS][2][KM_TILE];  // [group][turn]: minus the lse of the block's query rows
   __shared__ int s_see[KM_GROUPS][2][KM_TILE];                  // and the last key that each of them sees
-  __shared__ float s_sum[2 * KM_GROUPS][KM_TILE];               // the groups' sums (pass 1: maxima, then sums)
+  __shared__ float s_sum[2][KM_GROUPS][KM_TILE];                // the groups' maxima and sums (pass 2: sums, by turns)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;  // swizzled tiles start on 1024 bytes
   const uint32_t held = sbase, ring = sbase + C::OPERAND;
@@ -154,26 +164,52 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
   auto empty = [&](int s) { return bars + 8 * (C::STAGES + s); };
   auto acc_full = [&](int i) { return bars + 8 * (2 * C::STAGES + i); };
   auto acc_empty = [&](int i) { return bars + 8 * (2 * C::STAGES + KM_ACC + i); };
-  const uint32_t held_full = bars + 8 * (2 * C::STAGES + 2 * KM_ACC);
+  const uint32_t held_full = bars + 8 * (2 * C::STAGES + 2 * KM_ACC), held_empty = held_full + 8;
   if (tid == 0) {
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
     for (int i = 0; i < KM_ACC; ++i) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 128); }
     mbar_init(held_full, 1);
+    mbar_init(held_empty, 1);
     fence_barrier_init();
     tma_prefetch_desc(&qmap);
     tma_prefetch_desc(&kmap);
   }
   pdl_wait();
   pdl_launch();
-  if (warp == 0) {
-    const int index = blockIdx.x / a.HKV;
-    const int2 it = find_item(a.t.B, index, [&](int b) {
-      const SeqPages sp = seq_pages(a.t, b);
-      if (SUM) return (sp.ctx + KM_TILE - 1) / KM_TILE;
-      const int T = window_of(a, b, sp).T;
-      return (T + a.tokens - 1) / a.tokens;
-    });
-    if (lane == 0) s_item = it;
+  // the CTA's items, one warp to each: pass 1 has one per CTA, pass 2 every gridDim.x-th
+  if (warp < (SUM ? KM_ITEMS : 1)) {
+    MassItem it{};
+    const int64_t number = blockIdx.x + int64_t(warp) * gridDim.x;
+    it.b = -1;
+    if (number < int64_t(INT_MAX)) {
+      const int2 at = find_item(a.t.B, int(number) / a.HKV, [&](int b) {
+        const SeqPages sp = seq_pages(a.t, b);
+        if (SUM) return (sp.ctx + KM_TILE - 1) / KM_TILE;
+        const int T = window_of(a, b, sp).T;
+        return (T + a.tokens - 1) / a.tokens;
+      });
+      it.b = at.x;
+      it.index = at.y;
+    }
+    if (it.b >= 0) {
+      it.kvh = int(number) % a.HKV;
+      it.sp = seq_pages(a.t, it.b);
+      it.w = window_of(a, it.b, it.sp);
+      it.scale = mass_scale(a, it.kvh);
+      const Window w = it.w;
+      const int blocks = (w.T + a.tokens - 1) / a.tokens;
+      if (SUM) {
+        it.begin = min(blocks, max(0, it.index * KM_TILE - w.first) / a.tokens);  // the first that sees the tile's first key
+        it.n = blocks - it.begin;
+      } else {
+        it.index = blocks - 1 - it.index;  // the blocks that see most come first
+        const int last = min(w.T, (it.index + 1) * a.tokens) - 1, tiles = (w.first + last) / KM_TILE + 1;
+        const int per = (tiles + a.splits - 1) / a.splits;
+        it.begin = min(tiles, int(blockIdx.y) * per);
+        it.n = min(tiles, it.begin + per) - it.begin;
+      }
+    }
+    if (lane == 0) s_item[warp] = it;
   }
   // blocks of a.tokens tokens leave the last rows of an operand untouched: zeros there, so that nothing old is NaN
   const int block_rows = a.tokens * a.G;
@@ -187,43 +223,30 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
     fence_proxy_async();
   }
   __syncthreads();
-  const int b = s_item.x;
-  if (b < 0) return;  // fewer items than the grid's bound
+  if (s_item[0].b < 0) return;  // fewer items than the grid's bound
+  int items = 1;
+  while (SUM && items < KM_ITEMS && s_item[items].b >= 0) ++items;
+  if (tid == 0)
+    for (int k = 1; k < items; ++k) s_item[k].t0 = s_item[k - 1].t0 + s_item[k - 1].n;
   if (warp == 2) { tmem_alloc(smem_u32(&s_tmem), KM_ACC * KM_TILE); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
-  const int kvh = blockIdx.x % a.HKV;
-  const SeqPages sp = seq_pages(a.t, b);
-  const Window w = window_of(a, b, sp);
-  const int blocks = (w.T + a.tokens - 1) / a.tokens;
-  // the held operand, and the streamed ones: tiles or blocks number begin .. begin + n - 1
-  const int item = SUM ? s_item.y : blocks - 1 - s_item.y;  // pass 1: the blocks that see most come first
-  int begin, n;
-  if (SUM) {
-    begin = min(blocks, max(0, item * KM_TILE - w.first) / a.tokens);  // the first block that sees the tile's first key
-    n = blocks - begin;
-  } else {
-    const int last = min(w.T, (item + 1) * a.tokens) - 1, tiles = (w.first + last) / KM_TILE + 1;
-    const int per = (tiles + a.splits - 1) / a.splits;
-    begin = min(tiles, int(blockIdx.y) * per);
-    n = min(tiles, begin + per) - begin;
-  }
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
     const int boxes = KM_TILE / a.box_rows;
     // lane l: the row of the tensor map where box l of a tile starts, -1 = behind the end of the sequence
-    auto box_at = [&](int tile) -> int {
+    auto box_at = [&](const MassItem& it, int tile) -> int {
       const int pos = tile * KM_TILE + lane * a.box_rows;
-      if (lane >= boxes || pos >= sp.ctx) return -1;
-      if (a.copied) return kvh * (a.t.n_indices * a.t.P) + sp.first * a.t.P + pos;
-      const int e = a.t.page_of(pos), id = page_at(a.t, sp.first + e);
+      if (lane >= boxes || pos >= it.sp.ctx) return -1;
+      if (a.copied) return it.kvh * (a.t.n_indices * a.t.P) + it.sp.first * a.t.P + pos;
+      const int e = a.t.page_of(pos), id = page_at(a.t, it.sp.first + e);
       return (id < 0 ? 0 : id) * 2 * a.t.P + (pos - e * a.t.P);
     };
-    const int x0 = a.copied ? 0 : kvh * D;
-    auto load_keys = [&](int y, uint32_t dst, uint32_t bar) {
+    auto load_keys = [&](const MassItem& it, int y, uint32_t dst, uint32_t bar) {
+      const int x0 = a.copied ? 0 : it.kvh * D;
       const int there = __popc(__ballot_sync(0xffffffffu, y >= 0));
       if (lane == 0) mbar_expect_tx(bar, there * a.box_rows * 128 * C::PANELS);
       __syncwarp();
@@ -234,57 +257,82 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
                       x0 + (i % C::PANELS) * 64, row);
       }
     };
-    auto load_block = [&](int blk, uint32_t dst, uint32_t bar) {
+    auto load_block = [&](const MassItem& it, int blk, uint32_t dst, uint32_t bar) {
       if (lane == 0) mbar_expect_tx(bar, block_rows * 128 * C::PANELS);
       __syncwarp();
       if (lane < C::PANELS)
-        tma_load_3d(dst + lane * C::PANEL, &qmap, bar, lane * 64, kvh * a.G, w.q0 + blk * a.tokens);
+        tma_load_3d(dst + lane * C::PANEL, &qmap, bar, lane * 64, it.kvh * a.G, it.w.q0 + blk * a.tokens);
     };
-    if (SUM) load_keys(box_at(item), held, held_full);
-    else load_block(item, held, held_full);
-    int y = SUM ? 0 : box_at(begin), t = 0;
-    for (; t < n; ++t) {
-      const int s = t % C::STAGES, next = !SUM && t + 1 < n ? box_at(begin + t + 1) : -1;
-      if (!mbar_wait(empty(s), (t / C::STAGES & 1) ^ 1)) {
+    int t = 0, holds = 0;
+    bool ok = true;
+    int y_held = SUM ? box_at(s_item[0], s_item[0].index) : 0;  // looked up an item ahead
+    for (int k = 0; ok && k < items; ++k) {
+      const MassItem it = s_item[k];
+      const int y_now = y_held;
+      if (SUM && k + 1 < items) y_held = box_at(s_item[k + 1], s_item[k + 1].index);
+      if (SUM && it.n == 0) continue;  // a sequence without a window
+      if (SUM && !mbar_wait(held_empty, (holds & 1) ^ 1)) {
         atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x10);
         break;
       }
-      if (SUM) load_block(begin + t, ring + s * C::OPERAND, full(s));
-      else load_keys(y, ring + s * C::OPERAND, full(s));
-      y = next;
+      if (SUM) load_keys(it, y_now, held, held_full);
+      else load_block(it, it.index, held, held_full);
+      ++holds;
+      int y = SUM ? 0 : box_at(it, it.begin);
+      for (int j = 0; j < it.n; ++j, ++t) {
+        const int s = t % C::STAGES, next = !SUM && j + 1 < it.n ? box_at(it, it.begin + j + 1) : -1;
+        if (!mbar_wait(empty(s), (t / C::STAGES & 1) ^ 1)) {
+          atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x10);
+          ok = false;
+          break;
+        }
+        if (SUM) load_block(it, it.begin + j, ring + s * C::OPERAND, full(s));
+        else load_keys(it, y, ring + s * C::OPERAND, full(s));
+        y = next;
+      }
     }
     // no load is on its way when the block ends, whichever wait ran out
-    mbar_wait(held_full, 0);
+    if (holds) mbar_wait(held_full, (holds - 1) & 1);
     for (int k = max(0, t - C::STAGES); k < t; ++k) mbar_wait(full(k % C::STAGES), k / C::STAGES & 1);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
     if (elect_one()) {
-      bool ok = mbar_wait(held_full, 0);
-      if (!ok) atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
       // descriptors once: an offset in bytes / 16 is added to their address field (one thread issues all, instruction by
       // instruction: building a descriptor per MMA took longer than the MMA)
       const uint64_t held_desc = smem_desc(held, 16, 1024, 2), ring_desc = smem_desc(ring, 16, 1024, 2);
-      int t = 0;
-      for (; ok && t < n; ++t) {
-        const int s = t % C::STAGES, i = t % KM_ACC;
-        if (!mbar_wait(acc_empty(i), (t / KM_ACC & 1) ^ 1)) {
-          atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x20);
-          break;
-        }
-        if (!mbar_wait(full(s), t / C::STAGES & 1)) {
+      int t = 0, holds = 0;
+      bool ok = true;
+      for (int k = 0; ok && k < items; ++k) {
+        const int n = s_item[k].n;
+        if (SUM && n == 0) continue;
+        if (!mbar_wait(held_full, holds++ & 1)) {
           atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
           break;
         }
-        tc_fence_after();
-        const uint64_t streamed = ring_desc + s * (C::OPERAND / 16);
+        for (int j = 0; j < n; ++j, ++t) {
+          const int s = t % C::STAGES, i = t % KM_ACC;
+          if (!mbar_wait(acc_empty(i), (t / KM_ACC & 1) ^ 1)) {
+            atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x20);
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(full(s), t / C::STAGES & 1)) {
+            atomicOr(a.t.status, DS_WAIT_TIMEOUT | 0x40);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t streamed = ring_desc + s * (C::OPERAND / 16);
 #pragma unroll
-        for (int p = 0; p < C::PANELS; ++p)
+          for (int p = 0; p < C::PANELS; ++p)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 channels = 32 bytes of a panel's rows
-            tc_mma_bf16(tmem + i * KM_TILE, held_desc + (p * C::PANEL + k * 32) / 16,
-                        streamed + (p * C::PANEL + k * 32) / 16, (p | k) != 0);
-        tc_commit(empty(s));
-        tc_commit(acc_full(i));
+            for (int c = 0; c < 4; ++c)  // 16 channels = 32 bytes of a panel's rows
+              tc_mma_bf16(tmem + i * KM_TILE, held_desc + (p * C::PANEL + c * 32) / 16,
+                          streamed + (p * C::PANEL + c * 32) / 16, (p | c) != 0);
+          tc_commit(empty(s));
+          tc_commit(acc_full(i));
+        }
+        if (SUM && ok && k + 1 < items) tc_commit(held_empty);
       }
       // nor a product
       for (int k = max(0, t - KM_ACC); k < t; ++k) mbar_wait(acc_full(k % KM_ACC), k / KM_ACC & 1);
@@ -294,7 +342,6 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
     // ---------------------------------------------------------------- accumulators: group g takes every fourth one
     const int g = (warp - 4) / 4, row = (warp & 3) * 32 + lane;
     const uint32_t quarter = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const float scale = mass_scale(a, kvh);
     // false once a wait has run out (for the whole warp alike); the group's barriers are met all the same
     bool alive = true;
     auto wait_acc = [&](int t) {
@@ -310,6 +357,10 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
       mbar_arrive(acc_empty(t % KM_ACC));
     };
     if constexpr (!SUM) {
+      const MassItem it = s_item[0];
+      const Window w = it.w;
+      const int item = it.index, begin = it.begin, n = it.n;
+      const float scale = it.scale;
       const int tok = item * a.tokens + row / a.G;
       const bool real = row < block_rows && tok < w.T;
       const int see = w.first + tok, see_min = w.first + item * a.tokens;
@@ -359,31 +410,42 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
           }
         }
       }
-      s_sum[g][row] = m;
-      s_sum[KM_GROUPS + g][row] = l;
+      s_sum[0][g][row] = m;
+      s_sum[1][g][row] = l;
       asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
       if (g == 0 && real) {
 #pragma unroll
-        for (int i = 1; i < KM_GROUPS; ++i) m = fmaxf(m, s_sum[i][row]);
+        for (int i = 1; i < KM_GROUPS; ++i) m = fmaxf(m, s_sum[0][i][row]);
         const float base = m == -INFINITY ? 0.f : m;
         l = 0.f;
 #pragma unroll
-        for (int i = 0; i < KM_GROUPS; ++i) l += s_sum[KM_GROUPS + i][row] * ex2(s_sum[i][row] - base);
-        a.part[size_t(blockIdx.y) * a.T_total * a.HQ + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G] =
+        for (int i = 0; i < KM_GROUPS; ++i) l += s_sum[1][i][row] * ex2(s_sum[0][i][row] - base);
+        a.part[size_t(blockIdx.y) * a.T_total * a.HQ + size_t(w.q0 + tok) * a.HQ + size_t(it.kvh) * a.G + row % a.G] =
             make_float2(m, l);
       }
     } else {
-      const int key = item * KM_TILE + row;
       // the column whose lse this thread finds, a turn ahead, from the key ranges' maxima and sums; a query row with no
       // weight at all (every score -inf) and a column that stands for none get an infinite one: no weight
       const size_t rows = size_t(a.T_total) * a.HQ;
+      // the item that the column asked for last belongs to: where it ends, and what a column of it needs
+      int ahead = -1, ahead_end = 0, ahead_tok = 0, ahead_T = 0, ahead_first = 0;
+      const float2* ahead_part = nullptr;
       auto column = [&](int t, float& lse, int& see) {
-        const int tok = (begin + t) * a.tokens + row / a.G;
-        const bool real = t < n && row < block_rows && tok < w.T;
         lse = -INFINITY;
-        see = real ? w.first + tok : -1;
-        if (!real) return;
-        const float2* p = a.part + size_t(w.q0 + tok) * a.HQ + size_t(kvh) * a.G + row % a.G;
+        see = -1;
+        while (t >= ahead_end) {
+          if (++ahead >= items) return;
+          const MassItem& it = s_item[ahead];
+          ahead_end = it.t0 + it.n;
+          ahead_tok = (it.begin - it.t0) * a.tokens + row / a.G;
+          ahead_T = row < block_rows ? it.w.T : 0;
+          ahead_first = it.w.first;
+          ahead_part = a.part + size_t(it.w.q0) * a.HQ + size_t(it.kvh) * a.G + row % a.G;
+        }
+        const int tok = ahead_tok + t * a.tokens;
+        if (tok >= ahead_T) return;
+        see = ahead_first + tok;
+        const float2* p = ahead_part + size_t(tok) * a.HQ;
         float m = -INFINITY, l = 0.f;
         for (int s0 = 0; s0 < a.splits; s0 += 8) {
           float2 x[8];
@@ -401,52 +463,61 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
         if (l != 0.f) lse = -((m == -INFINITY ? 0.f : m) + log2f(l));
       };
       float lse;
-      int see;
-      column(g, lse, see);
-      float total = 0.f;
-      const uint64_t scale2 = pair(scale, scale);
-      for (int t = g; t < n; t += KM_GROUPS) {
-        const int turn = t / KM_GROUPS & 1;
-        s_lse[g][turn][row] = lse;
-        s_see[g][turn][row] = see;
-        column(t + KM_GROUPS, lse, see);
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
-        // the block's first token does not see the whole tile, or its last one is behind the window
-        const int tok0 = (begin + t) * a.tokens;
-        const bool masked = w.first + tok0 < item * KM_TILE + KM_TILE - 1 || tok0 + a.tokens > w.T;
-        if (!wait_acc(t)) continue;
-        uint64_t sum[2] = {0ull, 0ull};
+      int see, t = g;
+      column(t, lse, see);
+      for (int k = 0; k < items; ++k) {
+        const MassItem& it = s_item[k];
+        const int key = it.index * KM_TILE + row, end = it.t0 + it.n;
+        const int tok_t0 = (it.begin - it.t0) * a.tokens, T = it.w.T;
+        const int sees_all = it.index * KM_TILE + KM_TILE - 1 - it.w.first;  // from this token on a query sees the whole tile
+        const float scale = it.scale;
+        const uint64_t scale2 = pair(scale, scale);
+        float total = 0.f;
+        for (; t < end; t += KM_GROUPS) {
+          const int turn = t / KM_GROUPS & 1;
+          s_lse[g][turn][row] = lse;
+          s_see[g][turn][row] = see;
+          column(t + KM_GROUPS, lse, see);
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
+          // the block's first token does not see the whole tile, or its last one is behind the window
+          const int tok0 = tok_t0 + t * a.tokens;
+          const bool masked = tok0 < sees_all || tok0 + a.tokens > T;
+          if (!wait_acc(t)) continue;
+          uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll 1
-        for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
-          float v[32];
-          tmem_ld_x32(quarter + t % KM_ACC * KM_TILE + c0, v);
-          if (c0 == KM_TILE - 32) done(t);
-          if (masked) {
+          for (int c0 = 0; c0 < KM_TILE; c0 += 32) {
+            float v[32];
+            tmem_ld_x32(quarter + t % KM_ACC * KM_TILE + c0, v);
+            if (c0 == KM_TILE - 32) done(t);
+            if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (s_see[g][turn][c0 + i] >= key) total += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
-          } else {
+              for (int i = 0; i < 32; ++i)
+                if (s_see[g][turn][c0 + i] >= key) total += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&s_lse[g][turn][c0 + i]);
-              sum[0] = add2(sum[0], ex2_pair(fma2(pair(v[i], v[i + 1]), scale2, x.x)));
-              sum[1] = add2(sum[1], ex2_pair(fma2(pair(v[i + 2], v[i + 3]), scale2, x.y)));
+              for (int i = 0; i < 32; i += 4) {
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&s_lse[g][turn][c0 + i]);
+                sum[0] = add2(sum[0], ex2_pair(fma2(pair(v[i], v[i + 1]), scale2, x.x)));
+                sum[1] = add2(sum[1], ex2_pair(fma2(pair(v[i + 2], v[i + 3]), scale2, x.y)));
+              }
             }
           }
+          const float2 s2 = halves(add2(sum[0], sum[1]));
+          total += s2.x + s2.y;
         }
-        const float2 s2 = halves(add2(sum[0], sum[1]));
-        total += s2.x + s2.y;
-      }
-      s_sum[g][row] = total;
-      asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
-      if (g == 0 && key < sp.ctx) {
+        // the tile is done once all groups are; one of them, by turns, stores it while the others go on
+        s_sum[k & 1][g][row] = total;
+        asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
+        if (g == k % KM_GROUPS && key < it.sp.ctx) {
+          total = s_sum[k & 1][0][row];
 #pragma unroll
-        for (int i = 1; i < KM_GROUPS; ++i) total += s_sum[i][row];
-        const int e = a.t.page_of(key), page = page_at(a.t, sp.first + e);
-        if (page >= 0) {
-          float* dst = a.key_mass + (size_t(page) * a.t.P + (key - e * a.t.P)) * a.HKV + kvh;
-          if (a.accumulate) atomicAdd(dst, total);  // a page may be listed by several sequences
-          else *dst = total;
+          for (int i = 1; i < KM_GROUPS; ++i) total += s_sum[k & 1][i][row];
+          const int e = a.t.page_of(key), page = page_at(a.t, it.sp.first + e);
+          if (page >= 0) {
+            float* dst = a.key_mass + (size_t(page) * a.t.P + (key - e * a.t.P)) * a.HKV + it.kvh;
+            if (a.accumulate) atomicAdd(dst, total);  // a page may be listed by several sequences
+            else *dst = total;
+          }
         }
       }
     }
@@ -510,7 +581,16 @@ static int launch_mass(const MassArgs& a, const CUtensorMap& qmap, const CUtenso
                qmap, kmap, a);
     Q35_CUDA_LAUNCH_CHECK("attn.key_mass rows");
   }
-  launch_pdl(mass_kernel<D, true>, dim3(unsigned(tiles * a.HKV)), dim3(KM_THREADS), C::SMEM, stream, qmap, kmap, a);
+  // Short windows: a CTA per SM takes its tiles one after the other, so that what a tile waits for (tables, first loads,
+  // the last exponentials) is met while its neighbours work.  Long ones, 32 blocks of queries and more: a CTA per tile, so
+  // that the lengths even out (four prompts of up to 8192, 2 heads: 32 queries 29.8 us and 37.2, 300 queries 118 and 123;
+  // 2047 queries 646 and 620).
+  int64_t grid = tiles * a.HKV;
+  if (grid > sm_count() && blocks <= 32 * int64_t(a.t.B)) {
+    const int64_t least = (grid + KM_ITEMS - 1) / KM_ITEMS;
+    grid = least > sm_count() ? least : sm_count();
+  }
+  launch_pdl(mass_kernel<D, true>, dim3(unsigned(grid)), dim3(KM_THREADS), C::SMEM, stream, qmap, kmap, a);
   Q35_CUDA_LAUNCH_CHECK("attn.key_mass columns");
   return 0;
 }

@@ -349,6 +349,25 @@ def test_key_mass(fmt, D, HKV, G, P):
     assert q35.device_status() == 0
 
 
+@pytest.mark.parametrize("HKV,G,D,T", [(40, 1, 64, [3, 0, 130, 1]), (24, 8, 128, [20, 37, 0, 16]), (16, 6, 256, [5, 40, 64, 0])])
+def test_key_mass_of_many_tiles(HKV, G, D, T):
+    """several tiles to a CTA: of other sequences and heads, with windows of other lengths, and none"""
+    import ax_dsl_kernels_b200 as q35
+    ctxs, P = [1300, 400, 700, 1000], 64
+    cache, table, scales, g = make(ctxs, P, HKV, D, "bf16", 32)
+    cache, used = poison_behind(cache, table, P)
+    q = q_rows(sum(T), HKV * G, D, g, 2.0)
+    qo = torch.tensor([0, *torch.tensor(T).cumsum(0).tolist()], dtype=torch.int32)
+    old = torch.rand((cache.shape[0], P, HKV), generator=g)
+    for acc in (False, True):
+        ref, reach = olc.key_mass(q, cache, qo, *table, old, accumulate=acc)
+        gm = gpu(old)
+        q35.paged_key_mass(gpu(q), gpu(cache), gpu(qo), *gpu(table), gm, accumulate=acc)
+        check_mass(gm, ref, torch.zeros_like(old), reach, D, n_add=max(T) * G)
+        assert torch.equal(gm.cpu()[~used], old[~used])
+    assert q35.device_status() == 0
+
+
 @pytest.mark.parametrize("T", [1, 2, 17, 700])
 def test_key_mass_weights_sum_to_the_number_of_query_rows(T):
     import ax_dsl_kernels_b200 as q35
