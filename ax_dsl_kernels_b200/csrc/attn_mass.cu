@@ -17,7 +17,7 @@
 // owner and a fixed order, and nothing is exchanged but the groups' partial sums.
 // The groups' arithmetic is what takes longest to keep up: four warps per scheduler hide its latency, two numbers go to
 // an fma or add (f32x2), tiles that every row sees whole have a path without a mask.  (Two groups, a mask for every
-// tile, one number at a time: 273 us instead of 243 for 2047 queries over 8192 rows.  The held operand in tensor memory
+// tile, one number at a time: 273 us instead of 245 for 2047 queries over 8192 rows.  The held operand in tensor memory
 // and three groups: 239, but 44 instead of 37 for 32 queries over four prompts, whose one load per item it exposes.)
 //
 // A block holds the (token, head) pairs of floor(128 / G) tokens, fetched as one 3-D box; the keys come straight from the
