@@ -55,6 +55,7 @@ template <int D, int KVF>
 struct SparseCfg {
   static constexpr bool BYTE = KVF != 0;
   static constexpr int WARPS = 4;
+  static constexpr int TERMS = KVF == 1 ? 2 : 3;        // 16-bit numbers that make up a weight in the P V product
   static constexpr int SLOTS = 3;                       // half steps (32 rows of K or of V) per warp
   static constexpr int ROWB = D * (BYTE ? 1 : 2);
   static constexpr int CPR = ROWB / 16;                 // 16-byte chunks per row
@@ -131,7 +132,7 @@ __device__ __forceinline__ int flat_per_cta(const SparseArgs& a) {
 template <int D, int KVF, bool FLAT>
 __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KVF>::CTAS) sparse_decode_kernel(const SparseArgs a) {
   using C = SparseCfg<D, KVF>;
-  constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS;
+  constexpr int WARPS = C::WARPS, THREADS = 32 * WARPS, TERMS = C::TERMS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_part[SP_G * D];                        // this CTA's merged output, read by the cluster
   __shared__ float s_ml[2 * SP_G];                          // its maxima and sums, read by the cluster
@@ -419,9 +420,10 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
       m_run[h] = mn;
       ref[h] = base - LIFT;
     }
-    // bf16 / int8: P enters the P V product as two bf16 terms (p = hi + lo); one alone, 2^-8, would cost as much as the
-    // output's own rounding.  E4M3: one f16 term, 2^-11, an eighth of it (a second one: 58 -> 60 us for 32 sequences of up to 4161 rows).
-    uint32_t pb[2][2], pl[2][2];  // pl: unused for E4M3
+    // The weights meet V whole: p as three bf16 terms (24 bits) beside bf16 and int8 rows, as two f16 terms (22 bits) beside
+    // E4M3 ones.  (One f16 term rounded 4.8 % of the bf16 outputs the other way than the exact sum does, two 0.04 %, for
+    // 51.8 -> 53.4 us with 32 sequences of up to 4161 rows; two bf16 terms against three: 88.0 and 91.4 us for 64 x 4096 rows.)
+    uint32_t pb[TERMS][2][2];
     l_run[0] *= alpha[0];
     l_run[1] *= alpha[1];
 #pragma unroll
@@ -431,12 +433,19 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
         const float p0 = ex2(sc[h][2 * u] - ref[0]), p1 = ex2(sc[h][2 * u + 1] - ref[1]);
         l_run[0] += p0;
         l_run[1] += p1;
-        if constexpr (KVF == 1) {
-          pb[h][u] = movmatrix_trans(pack_f16(p0, p1));
-        } else {
-          const float h0 = round_bf16(p0), h1 = round_bf16(p1);
-          pb[h][u] = movmatrix_trans(pack_bf16(h0, h1));
-          pl[h][u] = movmatrix_trans(pack_bf16(p0 - h0, p1 - h1));
+        float left0 = p0, left1 = p1;  // of the weights, behind the terms so far
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          const uint32_t w = KVF == 1 ? pack_f16(left0, left1) : pack_bf16(left0, left1);
+          pb[t][h][u] = movmatrix_trans(w);
+          if constexpr (KVF == 1) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            left0 -= f.x;
+            left1 -= f.y;
+          } else {
+            left0 -= bf16lo(w);
+            left1 -= bf16hi(w);
+          }
         }
       }
     }
@@ -464,11 +473,10 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
             ldmatrix_x4_trans(rowa + h * SP_SUB * C::ROWB + ((ch ^ (key & C::SWZ)) << 4), f[m][0], f[m][1], f[m][2], f[m][3]);
           }
 #pragma unroll
-          for (int m = 0; m < MB; ++m)
-            mma_bf16_16816(oacc[m0 + m], f[m][0], f[m][1], f[m][2], f[m][3], pb[h][0], pb[h][1]);
+          for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-          for (int m = 0; m < MB; ++m)
-            mma_bf16_16816(oacc[m0 + m], f[m][0], f[m][1], f[m][2], f[m][3], pl[h][0], pl[h][1]);
+            for (int m = 0; m < MB; ++m)
+              mma_bf16_16816(oacc[m0 + m], f[m][0], f[m][1], f[m][2], f[m][3], pb[t][h][0], pb[t][h][1]);
         }
       }
     } else {
@@ -499,15 +507,19 @@ __global__ void __launch_bounds__(32 * SparseCfg<D, KVF>::WARPS, SparseCfg<D, KV
             x[2] = cvt_s8x2_bf16x2<0, 2>(r1, vc, vd); x[3] = cvt_s8x2_bf16x2<1, 3>(r1, vc, vd);
             x[4] = cvt_s8x2_bf16x2<0, 2>(r2, va, vb); x[5] = cvt_s8x2_bf16x2<1, 3>(r2, va, vb);
             x[6] = cvt_s8x2_bf16x2<0, 2>(r3, vc, vd); x[7] = cvt_s8x2_bf16x2<1, 3>(r3, vc, vd);
-            mma_bf16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[h][0], pb[h][1]);
-            mma_bf16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[h][0], pb[h][1]);
-            mma_bf16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pl[h][0], pl[h][1]);
-            mma_bf16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pl[h][0], pl[h][1]);
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+              mma_bf16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[t][h][0], pb[t][h][1]);
+              mma_bf16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[t][h][0], pb[t][h][1]);
+            }
           } else {
             x[0] = cvt_kv<0, 2>(r0); x[1] = cvt_kv<1, 3>(r0); x[2] = cvt_kv<0, 2>(r1); x[3] = cvt_kv<1, 3>(r1);
             x[4] = cvt_kv<0, 2>(r2); x[5] = cvt_kv<1, 3>(r2); x[6] = cvt_kv<0, 2>(r3); x[7] = cvt_kv<1, 3>(r3);
-            mma_f16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[h][0], pb[h][1]);
-            mma_f16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[h][0], pb[h][1]);
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+              mma_f16_16816(oacc[2 * mp], x[0], x[1], x[2], x[3], pb[t][h][0], pb[t][h][1]);
+              mma_f16_16816(oacc[2 * mp + 1], x[4], x[5], x[6], x[7], pb[t][h][0], pb[t][h][1]);
+            }
           }
         }
       }
