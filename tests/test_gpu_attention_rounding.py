@@ -86,3 +86,36 @@ def test_weights_meet_v_with_all_their_bits(fmt, D):
     tol = ref.abs() * 2.0 ** -8 + size * 2.0 ** -20
     assert ((got - ref).abs() <= tol).all(), f"worst {((got - ref).abs() / tol).max():.3g} of the tolerance"
     assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMT[:2] + FMT[3:])
+def test_long_sums_lose_nothing_on_the_way(fmt):
+    """16384 rows whose second half takes the first half's terms away again, at one CTA per (sequence, KV head): the output
+    is 0, and what comes out instead is what the sums lost while they rose and fell.
+
+    Tolerance: a warp adds up 128 steps, rounded to nearest, 2^-24 of running sums that are half their peak on average, and
+    the peaks are half of sum p |v|: 2^-19 of it; within a step six products, each cut off at 2^-23 of the step's own sum,
+    2^-20.  A rounding to nearest goes either way: the mean over 512 channels has to be 1 / 8 of that (the mean of 512
+    errors of one bound has a 75th of it as its deviation); one that always goes towards zero shows there."""
+    import ax_dsl_kernels_b200 as q35
+    HKV, D, P, n, B = 2, 256, 64, 16384, 80
+    g = torch.Generator().manual_seed(43)
+    k, v = torch.zeros((1, n, HKV, D), dtype=torch.float64), torch.zeros((1, n, HKV, D), dtype=torch.float64)
+    k[0, :n // 2, :, 0] = -torch.randint(0, 12, (n // 2, HKV), generator=g).double() / 8
+    k[0, ::32, :, 0] = 0.0  # the largest score is in every step: no rescaling
+    v[0, :n // 2] = stored(1 + torch.rand((n // 2, HKV, D), generator=g, dtype=torch.float64) * 0.9, fmt)[0]
+    k[0, n // 2:], v[0, n // 2:] = k[0, :n // 2], -v[0, :n // 2]
+    cache, (indptr, indices, last), scales = cache_of(k, v, P, fmt)
+    q = torch.zeros((1, HKV, D), dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    ref, _, size, _ = olc.sparse_decode(q, cache, indptr, indices, last, sm_scale=1.0, **scales)
+    assert (ref.abs() < 1e-12).all()
+    table = (torch.arange(B + 1, dtype=torch.int32) * (n // P), indices.repeat(B), last.repeat(B))  # all read the same pages
+    pages = torch.arange(n // P, dtype=torch.int32).expand(B, HKV, -1).contiguous()
+    got = q35.paged_attention_sparse(gpu(q.expand(B, -1, -1).contiguous()), gpu(cache), *gpu(table), gpu(pages), sm_scale=1.0,
+                                     **gpu_scales(scales)).double().cpu()
+    tol = size * (2.0 ** -19 + 2.0 ** -20)
+    assert torch.equal(got, got[:1].expand_as(got))
+    assert (got[:1].abs() <= tol).all(), f"worst {(got[:1].abs() / tol).max():.3g} of the tolerance"
+    assert (got[0] / tol[0]).mean().abs() <= 1 / 8, f"mean {(got[0] / tol[0]).mean():.3g} of the tolerance"
+    assert q35.device_status() == 0
