@@ -494,6 +494,10 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
               for (int i = 0; i < 32; ++i)
                 if (s_see[g][turn][c0 + i] >= key) total += ex2(fmaf(v[i], scale, s_lse[g][turn][c0 + i]));
             } else {
+              if (c0 + 32 > block_rows) {  // the rows of zeros behind the block: their product with an infinite key is NaN
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = c0 + i < block_rows ? v[i] : 0.f;
+              }
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
                 const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&s_lse[g][turn][c0 + i]);

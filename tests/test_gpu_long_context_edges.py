@@ -1,0 +1,49 @@
+"""The long-context roles where they can go wrong: infinite keys beside every head group, refused windows, tables and counts
+at their limits, scratch memory and streams.
+
+Tolerances: those of test_gpu_long_context.py, with the share that a score's error has kept to the weight that is added:
+w (2 (D + 4) 2^-23 R + 2^-18 + terms 2^-23) for a weight w that is a sum of `terms` exponentials, and 2^-24 of the result for
+every addition to what the row held."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from oracle import long_context as olc  # noqa: E402
+from test_gpu_long_context import check_out, gpu, gpu_scales, make, poison_behind, q_rows, random_pages  # noqa: E402, F401
+
+
+def check_added(got, ref, old, reach, D, terms, adds=1):
+    """got against ref = old + weights, row by row"""
+    got, old = got.double().cpu(), old.double()
+    w = (ref - old).abs()
+    tol = w * (2 * (D + 4) * 2.0 ** -23 * reach + 2.0 ** -18 + terms * 2.0 ** -23) + adds * 2.0 ** -24 * (old.abs() + w) + 1e-30
+    bad = ~((got - ref).abs() <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, worst {((got - ref).abs() / tol).max():.3g} of the tolerance"
+
+
+def windows(T):
+    return torch.tensor([0, *torch.tensor(T).cumsum(0).tolist()], dtype=torch.int32)
+
+
+# ---------------------------------------------------------------------------------------------------- window weights
+@pytest.mark.parametrize("G,D", [(3, 64), (5, 128), (6, 256), (7, 64), (48, 128), (43, 64), (8, 128)])
+def test_key_mass_beside_keys_masked_by_infinity(G, D):
+    """head groups that fill a block of 128 query rows and that do not; tiles that the whole block sees"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, ctxs, T = 64, 2, [700, 400], [60, 45]
+    cache, table, _, g = make(ctxs, P, HKV, D, "bf16", 51)
+    q = q_rows(sum(T), HKV * G, D, g)
+    q[:, :, 0] = 1.0
+    for b in range(2):
+        page, row = olc._places(*table, P, b)
+        for i in (0, 3, 200, 300, ctxs[b] - 2):
+            cache[page[i], 0, row[i]] = 0.0
+            cache[page[i], 0, row[i], :, 0] = float("-inf")
+    old = torch.zeros((cache.shape[0], P, HKV))
+    ref, reach = olc.key_mass(q, cache, windows(T), *table, old)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows(T)), *gpu(table), gm)
+    assert not ref.isnan().any() and not gm.isnan().any()
+    check_added(gm, ref, old, reach, D, max(T) * G)
+    assert q35.device_status() == 0
