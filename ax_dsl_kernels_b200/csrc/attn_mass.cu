@@ -52,15 +52,16 @@ struct MassArgs {
   int copied;                  // keys come from the bf16 copy [HKV, n_indices P, D]
 };
 
-// the window of sequence b: tokens q0 .. q0 + T - 1 of q, the first of them at position `first`; T = 0 if there is none
-struct Window { int q0, T, first; };
+// the window of sequence b: tokens q0 .. q0 + T - 1 of q, the first of them at position `first`; T = 0 if there is none, and
+// `refused` if what the table says is no window of this sequence: recorded, and its weights stay as they are
+struct Window { int q0, T, first; bool refused; };
 __device__ __forceinline__ Window window_of(const MassArgs& a, int b, const SeqPages& sp) {
   const int q0 = a.qo_indptr[b], q1 = a.qo_indptr[b + 1];
   if (q0 < 0 || q1 < q0 || q1 > a.T_total || q1 - q0 > sp.ctx) {  // the cache must hold the window's own rows
     atomicOr(a.t.status, DS_BAD_TOKEN);
-    return {0, 0, 0};
+    return {0, 0, 0, true};
   }
-  return {q0, q1 - q0, sp.ctx - (q1 - q0)};
+  return {q0, q1 - q0, sp.ctx - (q1 - q0), false};
 }
 
 __device__ __forceinline__ float mass_scale(const MassArgs& a, int kvh) {
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
         // the tile is done once all groups are; one of them, by turns, stores it while the others go on
         s_sum[k & 1][g][row] = total;
         asm volatile("bar.sync %0, %1;" ::"n"(1 + KM_GROUPS), "n"(128 * KM_GROUPS) : "memory");
-        if (g == k % KM_GROUPS && key < it.sp.ctx) {
+        if (g == k % KM_GROUPS && key < it.sp.ctx && !it.w.refused) {
           total = s_sum[k & 1][0][row];
 #pragma unroll
           for (int i = 1; i < KM_GROUPS; ++i) total += s_sum[k & 1][i][row];

@@ -47,3 +47,32 @@ def test_key_mass_beside_keys_masked_by_infinity(G, D):
     assert not ref.isnan().any() and not gm.isnan().any()
     check_added(gm, ref, old, reach, D, max(T) * G)
     assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("qo", [[0, 4, 40, 43], [0, 4, 3, 3], [0, 4, 50, 60], [0, 4, -1, 3]])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_refused_window_leaves_its_sequence_as_it_was(qo, accumulate):
+    """a window longer than its sequence, one that ends before it begins, rows behind q: recorded, and the weights of that
+    sequence stay; those of the others are right"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, ctxs = 16, 2, 4, 64, [200, 30, 150]
+    cache, table, _, g = make(ctxs, P, HKV, D, "bf16", 52)
+    qo = torch.tensor(qo, dtype=torch.int32)
+    fine = [b for b in range(3) if 0 <= qo[b] <= qo[b + 1] <= 43 and qo[b + 1] - qo[b] <= ctxs[b]]
+    assert 0 in fine and 1 not in fine
+    q = q_rows(43, HKV * G, D, g, 2.0)
+    old = torch.rand((cache.shape[0], P, HKV), generator=g)
+    want, base, reach = old.double(), old.clone(), 0.0
+    for b in fine:
+        one = (table[0][[b, b + 1]] - table[0][b], table[1][int(table[0][b]):int(table[0][b + 1])], table[2][b:b + 1])
+        want, r = olc.key_mass(q[int(qo[b]):int(qo[b + 1])], cache, windows([int(qo[b + 1] - qo[b])]), *one, want, accumulate)
+        reach = max(reach, r)
+        if not accumulate:
+            base[olc._places(*one, P, 0)] = 0.0
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(qo), *gpu(table), gm, accumulate=accumulate)
+    assert q35.device_status() & 8
+    for b in set(range(3)) - set(fine):
+        page, row = olc._places(*table, P, b)
+        assert torch.equal(gm.cpu()[page, row], old[page, row])
+    check_added(gm, want, base, reach, D, 43 * G)
