@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsArgs a) {
   }
   const int b = blockIdx.x / a.per_seq;
   const SeqPages sp = seq_pages(a.t, b);
-  for (int i = max(0, a.first_page[b]) + int(blockIdx.x) % a.per_seq; i < sp.n; i += a.per_seq) {
+  const int from = min(max(0, a.first_page[b]), sp.n);  // whatever the tensor holds: sums of it stay below 2^31
+  for (int i = from + int(blockIdx.x) % a.per_seq; i < sp.n; i += a.per_seq) {
     const int page = page_at(a.t, sp.first + i);
     if (page >= 0) page_bounds_one<KVF>(a, page, min(a.t.P, sp.ctx - i * a.t.P), s_red);
   }

@@ -76,3 +76,17 @@ def test_a_refused_window_leaves_its_sequence_as_it_was(qo, accumulate):
         page, row = olc._places(*table, P, b)
         assert torch.equal(gm.cpu()[page, row], old[page, row])
     check_added(gm, want, base, reach, D, 43 * G)
+
+
+def test_first_pages_behind_the_end():
+    """page_key_bounds from a page on that no sequence has, up to the largest number there is: nothing is looked at"""
+    import ax_dsl_kernels_b200 as q35
+    ctxs = [100, 1, 0, 64, 200]
+    cache, table, _, g = make(ctxs, 16, 2, 64, "bf16", 53)
+    old = torch.randn((cache.shape[0], 2, 2, 64), generator=g).to(torch.bfloat16)
+    for first in ([2 ** 31 - 1] * 5, [7, 2 ** 31 - 1, 0, 2 ** 31 - 3, 2 ** 30], [2 ** 31 - 1, -2 ** 31, 5, 3, 2 ** 31 - 2]):
+        first = torch.tensor(first, dtype=torch.int32)
+        ref = olc.page_bounds(cache, *table, old, first_page=first)
+        got = q35.page_key_bounds(gpu(cache), *gpu(table), gpu(old), first_page=gpu(first))
+        assert torch.equal(got.cpu(), ref)
+    assert q35.device_status() == 0
