@@ -1,6 +1,8 @@
 // C ABI of the library: role registry, by-name binding, validation (see include/q35b200.h).
 #include "abi.h"
 #include <atomic>
+#include <exception>
+#include <map>
 #include <mutex>
 #include <string>
 #include <unordered_map>
@@ -275,6 +277,27 @@ static const RoleDef kRoles[] = {
 };
 static const int kNumRoles = int(sizeof(kRoles) / sizeof(kRoles[0]));
 
+// One lock per (device, stream), held while a call is issued.  Roles of several launches hand results from one to the next
+// in the workspace, and host threads that share a stream share its workspace: nothing of another call may come between.
+// Calls on different streams do not wait for one another.
+static std::mutex& issue_lock(cudaStream_t stream) {
+  static std::mutex guard;
+  static std::map<std::pair<int, cudaStream_t>, std::mutex> locks;
+  int dev = -1;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(guard);
+  return locks[{dev, stream}];
+}
+
+// what a C++ exception becomes at the C entries: hosts in other languages cannot catch one
+static int failed_by(const char* what) noexcept {
+  try {
+    return fail(Q35_ERR_CUDA, "host exception: %s", what);
+  } catch (...) {  // not even memory for the text
+    return Q35_ERR_CUDA;
+  }
+}
+
 static const RoleDef* find_role(const char* role) {
   if (!role) return nullptr;
   for (int i = 0; i < kNumRoles; ++i)
@@ -297,7 +320,12 @@ int q35_run(const char* role, const q35_io* ios, int n_io, void* stream) {
   // a status code here and never a null pointer inside a kernel
   if (!device_info()) return Q35_ERR_CUDA;
   Call c{ios, n_io, static_cast<cudaStream_t>(stream), false, 0};
-  return r->run(c);
+  try {
+    std::lock_guard<std::mutex> lock(issue_lock(c.stream));
+    return r->run(c);
+  } catch (const std::exception& e) {
+    return failed_by(e.what());
+  }
 }
 
 int64_t q35_workspace_bytes(const char* role, const q35_io* ios, int n_io) {
@@ -305,7 +333,12 @@ int64_t q35_workspace_bytes(const char* role, const q35_io* ios, int n_io) {
   const RoleDef* r = find_role(role);
   if (!r) return -int64_t(fail(Q35_ERR_ROLE, "unknown role '%s'", role ? role : "(null)"));
   Call c{ios, n_io, nullptr, true, 0};
-  int st = r->run(c);
+  int st;
+  try {
+    st = r->run(c);
+  } catch (const std::exception& e) {
+    st = failed_by(e.what());
+  }
   if (st) return -int64_t(st);
   return c.ws_need;
 }

@@ -65,7 +65,8 @@ enum q35_status {
 /* Run one kernel role with tensors bound by name on `stream` (a cudaStream_t; NULL = default stream).
  * Replaces AX_ENGINE_RunSync(handle, &io) (tools/board/axrun.cc:104-110) and the Python launch
  * kernel[cores](*[case[n] for n in order(fn)]) (models/qwen35_2b/whole/src/q35_layer_mc.py:915-916).
- * Validates names, dtypes, byte counts and shapes before anything is enqueued; returns a q35_status. */
+ * Validates names, dtypes, byte counts and shapes before anything is enqueued; returns a q35_status.
+ * Host threads may share a stream and its workspace: calls on one stream are issued one behind the other. */
 int q35_run(const char* role, const q35_io* ios, int n_io, void* stream);
 
 /* Scratch bytes the role needs for these shapes (0 if none); negative q35_status on a contract error.

@@ -90,3 +90,53 @@ def test_first_pages_behind_the_end():
         got = q35.page_key_bounds(gpu(cache), *gpu(table), gpu(old), first_page=gpu(first))
         assert torch.equal(got.cpu(), ref)
     assert q35.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------- host threads
+@pytest.mark.parametrize("role", ["key_mass", "key_mass int8", "all pages", "evict"])
+def test_two_threads_on_one_stream(role):
+    """roles of several launches, from two host threads whose calls share a stream and its scratch: every call's numbers are
+    those that it gives alone"""
+    import threading
+
+    import ax_dsl_kernels_b200 as q35
+    fmt = "int8" if "int8" in role else "bf16"
+    HKV, G, D, P, ctxs = (16, 1, 64, 64, [57344]) if role == "all pages" else (2, 6, 128, 64, [900, 300, 77])
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 54)
+    gc, gt, gs = gpu(cache), gpu(table), gpu_scales(scales)
+    T, n = [20, 33, 5], 40
+    qo = gpu(windows(T))
+    rows = sum(T) if "key_mass" in role else len(ctxs)
+    qs = [gpu(q_rows(rows, HKV * G, D, g, 2.0)) for _ in range(2)]
+    masses = [torch.rand((cache.shape[0], P, HKV), generator=g).cuda() for _ in range(2)]
+
+    def call(i):
+        if role == "all pages":
+            return q35.paged_attention_sparse(qs[i], gc, *gt)
+        if role == "evict":
+            mine, mass = caches[i].pop(), masses[i].clone()
+            return torch.cat([q35.evict_keys(mine, mass, *gt, 200, keep_last=9).float().flatten(), mine.float().flatten(), mass.flatten()])
+        gm = torch.zeros_like(masses[0])
+        return q35.paged_key_mass(qs[i], gc, qo, *gt, gm, **gs)
+
+    caches = [[gc.clone() for _ in range(n + 1)] for _ in range(2)] if role == "evict" else None
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    got, errors, start = [[], []], [], threading.Barrier(2)
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(n):
+                got[i].append(call(i))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for i in range(2):
+        assert len(got[i]) == n and all(torch.equal(x, want[i]) for x in got[i])
+    assert q35.device_status() == 0
