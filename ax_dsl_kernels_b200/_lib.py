@@ -115,9 +115,18 @@ def _workspace(dev, nbytes, stream):
 
 
 def _scratch(dev, nbytes, stream):
-    """(address, owner) of a call's workspace.  While a CUDA graph is being captured it comes from the graph's own memory:
-    a graph must not hold the address of a buffer that a later, larger call replaces, nor share one with another graph
-    that may be replayed beside it."""
+    """(address, owner) of a call's workspace on `stream`.  While that stream captures a CUDA graph it comes from the graph's
+    own memory: a graph must not hold the address of a buffer that a later, larger call replaces, nor share one with
+    another graph that may be replayed beside it.  (torch's captures: a host that captures by other means brings its own
+    workspace.)"""
+    if stream != _raw_stream(dev) or dev != torch.cuda.current_device():
+        # whether it captures, where the memory comes from and when it may go to somebody else are the stream's own matter
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, dev) if stream else torch.cuda.default_stream(dev)):
+            return _scratch_here(dev, nbytes, stream)
+    return _scratch_here(dev, nbytes, stream)
+
+
+def _scratch_here(dev, nbytes, stream):
     if torch.cuda.is_current_stream_capturing():
         own = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", dev))
         return own.data_ptr(), own

@@ -1,0 +1,77 @@
+"""The Python host's side of a call without a GPU: where scratch memory comes from."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+from ax_dsl_kernels_b200 import _lib
+
+
+class FakeCuda:
+    """two devices, streams by handle (0: the default one), some of them capturing; records what is allocated where"""
+
+    def __init__(self, monkeypatch, capturing=()):
+        self.dev, self.stream, self.capturing, self.made = 0, {0: 0, 1: 0}, set(capturing), []
+        for name, f in (("current_device", lambda: self.dev),
+                        ("is_current_stream_capturing", lambda: (self.dev, self.stream[self.dev]) in self.capturing),
+                        ("ExternalStream", self.external), ("default_stream", lambda d: types.SimpleNamespace(handle=0, dev=d)),
+                        ("stream", self.use)):
+            monkeypatch.setattr(torch.cuda, name, f)
+        monkeypatch.setattr(torch, "empty", self.empty)
+        monkeypatch.setattr(_lib, "_raw_stream", lambda d: self.stream[d])
+        monkeypatch.setattr(_lib, "_ws_cache", {})
+
+    @staticmethod
+    def external(handle, device):
+        assert handle, "handle 0 would name a stream of the pool"
+        return types.SimpleNamespace(handle=handle, dev=device)
+
+    @contextlib.contextmanager
+    def use(self, s):
+        old = self.dev, self.stream[s.dev]
+        self.dev, self.stream[s.dev] = s.dev, s.handle
+        try:
+            yield
+        finally:
+            self.dev, self.stream[s.dev] = old
+
+    def empty(self, n, dtype=None, device=None):
+        self.made.append((device.index, self.stream[device.index], n))
+        address = 4096 * len(self.made)
+        return types.SimpleNamespace(numel=lambda: n, data_ptr=lambda: address)
+
+
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("dev,handle", [(0, 0), (0, 7), (1, 0), (1, 7)])
+@pytest.mark.parametrize("current", [0, 5])
+def test_scratch_belongs_to_the_stream_of_the_call(monkeypatch, dev, handle, current):
+    cuda = FakeCuda(monkeypatch)
+    cuda.stream[0] = current
+    at, _ = _lib._scratch(dev, 10, handle)
+    assert cuda.made == [(dev, handle, MB)]
+    assert _lib._scratch(dev, MB, handle)[0] == at and len(cuda.made) == 1  # kept
+    assert _lib._scratch(dev, MB + 1, handle)[0] != at
+    assert cuda.made[1:] == [(dev, handle, MB + 1)]  # the old buffer goes back to this stream's memory too
+    assert (cuda.dev, cuda.stream[0]) == (0, current)
+
+
+@pytest.mark.parametrize("dev,handle,current", [(0, 7, 0), (0, 7, 5), (1, 7, 0), (1, 7, 7), (0, 5, 5)])
+def test_a_capture_on_the_calls_stream_takes_the_graphs_memory(monkeypatch, dev, handle, current):
+    """whatever stream and device are current"""
+    cuda = FakeCuda(monkeypatch, capturing=[(dev, handle)])
+    cuda.stream[dev] = current
+    _lib._scratch(dev, 10, handle)
+    _lib._scratch(dev, 20, handle)
+    assert cuda.made == [(dev, handle, 10), (dev, handle, 20)] and not _lib._ws_cache
+
+
+@pytest.mark.parametrize("handle", [0, 7])
+def test_a_capture_on_another_stream_is_no_matter(monkeypatch, handle):
+    """the current stream captures, the call goes elsewhere: its buffer is that stream's, not the graph's"""
+    cuda = FakeCuda(monkeypatch, capturing=[(0, 5)])
+    cuda.stream[0] = 5
+    at = _lib._scratch(0, 10, handle)[0]
+    assert cuda.made == [(0, handle, MB)] and _lib._ws_cache[0, handle][1] == at

@@ -140,3 +140,65 @@ def test_two_threads_on_one_stream(role):
     for i in range(2):
         assert len(got[i]) == n and all(torch.equal(x, want[i]) for x in got[i])
     assert q35.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------- streams by handle
+def handle_case(seed):
+    cache, table, _, g = make([700, 900], 64, 2, 128, "bf16", seed)
+    return gpu(cache), dict(zip(("indptr", "indices", "last_page_len"), gpu(table))), gpu(q_rows(2, 16, 128, g, 2.0))
+
+
+@pytest.mark.parametrize("current_captures", [False, True])
+def test_capture_of_a_call_on_a_stream_by_its_handle(current_captures):
+    """the stream named by the handle captures, the current one does not, or captures the same graph: scratch is the graph's.
+    Later calls on that stream need more and write over what is not"""
+    import ax_dsl_kernels_b200 as q35
+    from ax_dsl_kernels_b200 import _lib
+    gc, gt, q = handle_case(55)
+    out, gm = torch.empty_like(q), torch.zeros((gc.shape[0], 64, 2), device="cuda")
+    want, wm = torch.empty_like(q), torch.zeros_like(gm)
+    q35.run("attn.sparse_decode", q=q, paged_kv_cache=gc, **gt, out=want, key_mass=wm)
+    origin, side, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=origin):
+        if current_captures:  # fork
+            side.wait_stream(origin)
+            target, current = side, origin
+        else:
+            target, current = origin, torch.cuda.Stream()
+        with torch.cuda.stream(current):
+            q35.run("attn.sparse_decode", target.cuda_stream, q=q, paged_kv_cache=gc, **gt, out=out, key_mass=gm)
+        if current_captures:
+            origin.wait_stream(side)
+    assert (0, target.cuda_stream) not in _lib._ws_cache
+    with torch.cuda.stream(target):
+        for n in (1, 40):
+            ids = torch.randint(0, 32, (64 * n, 4), dtype=torch.int32, device="cuda")
+            q35.moe_permute(ids, torch.rand((64 * n, 4), device="cuda"), 32, 16)
+        junk = [torch.full((1 << 18,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(gm, wm) and len(junk) == 8
+
+
+def test_scratch_that_grows_on_a_stream_by_its_handle():
+    """calls of growing size on another stream, with nothing waited for, while the current stream allocates and writes: the
+    buffers that were outgrown stay the other stream's"""
+    import ax_dsl_kernels_b200 as q35
+    side, P, HKV, D = torch.cuda.Stream(), 64, 2, 128
+    cases = []
+    for i, ctx in enumerate((2000, 20000, 40000, 80000)):
+        cache, table, _, g = make([ctx], P, HKV, D, "bf16", 56 + i)
+        t = dict(zip(("indptr", "indices", "last_page_len"), gpu(table)), q=gpu(q_rows(1, 16, D, g, 2.0)), paged_kv_cache=gpu(cache))
+        outs = [[torch.empty_like(t["q"]), torch.zeros((cache.shape[0], P, HKV), device="cuda")] for _ in range(2)]
+        q35.run("attn.sparse_decode", **t, out=outs[0][0], key_mass=outs[0][1])
+        cases.append((t, outs))
+    torch.cuda.synchronize()
+    for t, outs in cases:
+        q35.run("attn.sparse_decode", side.cuda_stream, **t, out=outs[1][0], key_mass=outs[1][1])
+        for n in (1 << 20, 1 << 21, 1 << 23):
+            torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for _, (a, b) in cases:
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert q35.device_status() == 0
