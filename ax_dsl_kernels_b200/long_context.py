@@ -27,11 +27,14 @@ def _keep_pair(first, last, device):
         raise ValueError("keep_first and keep_last count pages or rows: not negative")
     key = (int(first), int(last), device.index)
     t = _keep.get(key)
-    if t is None and torch.cuda.is_current_stream_capturing():
-        t = torch.full((2,), int(first), dtype=torch.int32, device=device)
-        t[1:].fill_(int(last))
-    elif t is None:
-        t = _keep[key] = torch.tensor([int(first), int(last)], dtype=torch.int32, device=device)
+    if t is not None:
+        return t
+    with torch.cuda.device(device.index if device.type == "cuda" else -1):  # the device whose stream the call goes to
+        if torch.cuda.is_current_stream_capturing():
+            t = torch.full((2,), int(first), dtype=torch.int32, device=device)
+            t[1:].fill_(int(last))
+        else:
+            t = _keep[key] = torch.tensor([int(first), int(last)], dtype=torch.int32, device=device)
     return t
 
 

@@ -75,3 +75,34 @@ def test_a_capture_on_another_stream_is_no_matter(monkeypatch, handle):
     cuda.stream[0] = 5
     at = _lib._scratch(0, 10, handle)[0]
     assert cuda.made == [(0, handle, MB)] and _lib._ws_cache[0, handle][1] == at
+
+
+@pytest.mark.parametrize("current,capturing", [(0, [(1, 0)]), (0, [(0, 0)]), (1, [(1, 0)]), (1, [])])
+def test_counts_first_used_in_a_capture_on_another_device(monkeypatch, current, capturing):
+    """(first, last) pairs of select_pages and evict_keys: copied from the host and kept, or set by the graph that the tensors'
+    device captures"""
+    from ax_dsl_kernels_b200 import long_context as lc
+    cuda = FakeCuda(monkeypatch, capturing)
+    cuda.dev = current
+
+    @contextlib.contextmanager
+    def device(d):
+        old, cuda.dev = cuda.dev, d
+        yield
+        cuda.dev = old
+
+    class Filled:
+        def __getitem__(self, _):
+            return self
+
+        def fill_(self, _):
+            made.append("set by the graph")
+
+    made = []
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch, "tensor", lambda *a, **k: made.append("copied"))
+    monkeypatch.setattr(torch, "full", lambda *a, **k: Filled())
+    monkeypatch.setattr(lc, "_keep", {})
+    lc._keep_pair(6, 2, torch.device("cuda", 1))
+    assert made == ["set by the graph" if (1, 0) in capturing else "copied"]
+    assert bool(lc._keep) == ((1, 0) not in capturing) and cuda.dev == current
