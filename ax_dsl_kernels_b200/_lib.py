@@ -201,6 +201,8 @@ def _fast_run():
         from . import _bind
     except ImportError:
         return run_checked
+    if getattr(_bind, "built_for", None) != torch.__version__:  # it would read another torch's tensors
+        return run_checked
     L = lib()
     address = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
     _bind.init(address(L.q35_run), address(L.q35_workspace_bytes), run_checked, _scratch, _check)

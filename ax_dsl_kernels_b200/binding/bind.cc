@@ -138,4 +138,9 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, kMethods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__bind() { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__bind() {
+  PyObject* m = PyModule_Create(&kModule);
+  // the torch whose object layouts this file was compiled with: the host compares it before the first call
+  if (m && PyModule_AddStringConstant(m, "built_for", Q35_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

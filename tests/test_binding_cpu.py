@@ -106,3 +106,69 @@ def test_counts_first_used_in_a_capture_on_another_device(monkeypatch, current, 
     lc._keep_pair(6, 2, torch.device("cuda", 1))
     assert made == ["set by the graph" if (1, 0) in capturing else "copied"]
     assert bool(lc._keep) == ((1, 0) not in capturing) and cuda.dev == current
+
+
+# ------------------------------------------------------------------------------------------- the fast path and its build
+def test_the_fast_path_of_another_torch_is_not_used(monkeypatch):
+    import sys
+
+    import ax_dsl_kernels_b200 as q35
+    other = types.SimpleNamespace(built_for="1.0.0", init=lambda *a: pytest.fail("initialised"), run=None)
+    monkeypatch.setitem(sys.modules, "ax_dsl_kernels_b200._bind", other)
+    monkeypatch.setattr(q35, "_bind", other, raising=False)
+    assert _lib._fast_run() is _lib.run_checked
+
+
+def test_the_fast_path_is_built_for_this_torch():
+    _bind = pytest.importorskip("ax_dsl_kernels_b200._bind")
+    assert _bind.built_for == torch.__version__
+    assert _lib._fast_run() is _bind.run
+
+
+def build_in(monkeypatch, tmp_path, compiler):
+    from ax_dsl_kernels_b200 import build
+    source = tmp_path / "bind.cc"
+    source.write_text("")
+    monkeypatch.setattr(build, "HERE", str(tmp_path))
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    monkeypatch.setattr(build, "BIND", str(tmp_path / "_bind.this.so"))
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    return lambda **k: build.binding([str(source)], **k)
+
+
+def test_a_binding_that_does_not_compile_is_a_warning(monkeypatch, tmp_path):
+    binding = build_in(monkeypatch, tmp_path, lambda *a, **k: types.SimpleNamespace(returncode=1, stdout="", stderr="no such header"))
+    (tmp_path / "_bind.this.so").write_text("of an older torch")
+    with pytest.warns(UserWarning, match="no such header"):
+        binding()
+    assert not (tmp_path / "_bind.this.so").exists()  # nothing old is left to be imported
+
+    def no_compiler(*a, **k):
+        raise FileNotFoundError("g++")
+
+    binding = build_in(monkeypatch, tmp_path, no_compiler)
+    with pytest.warns(UserWarning, match="g[+][+]"):
+        binding()
+
+
+def test_another_torch_makes_the_binding_stale(monkeypatch, tmp_path):
+    built = []
+
+    def compiler(cmd, **k):
+        built.append(torch.__version__)
+        assert f'-DQ35_BUILT_FOR="{torch.__version__}"' in cmd
+        (tmp_path / "_bind.this.so").write_text("")
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    binding = build_in(monkeypatch, tmp_path, compiler)
+    (tmp_path / "_bind.so").write_text("for any Python")
+    here = torch.__version__
+    binding()
+    binding()
+    assert built == [here] and not (tmp_path / "_bind.so").exists()
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    binding()
+    binding()
+    assert built == [here, "99.0"]
+    binding(force=True)
+    assert len(built) == 3
