@@ -86,7 +86,9 @@ def paged_attention_sparse(q, paged_kv_cache, indptr, indices, last_page_len, pa
     gives them (None: all pages).  key_mass [pages, P, HKV] fp32, when given, gets the softmax weight of every attended
     row added, summed over the query heads of the row's KV head.  k_new / v_new [B, HKV, D]: the current token, attended
     to from its own rows whatever the pages; with key_mass, cache_location [B, 2] says where its own weight is stored
-    (stored, not added: the row is new).  Unlike paged_attention_decode nothing is written into the cache.
+    (stored, not added: the row is new; the table does not hold it yet).  Without them, a row that is new in the table
+    starts from whatever its place in key_mass held -- after an eviction or in a page used again, another row's weight --
+    and the caller clears it first.  Unlike paged_attention_decode nothing is written into the cache.
     A row without any page and without a current token gives zeros.  At most 8 query heads per KV head, head_dim 64, 128
     or 256, page size a multiple of 16.  Formats and scales as in paged_attention_decode."""
     out = torch.empty_like(q) if out is None else out

@@ -202,3 +202,66 @@ def test_scratch_that_grows_on_a_stream_by_its_handle():
     for _, (a, b) in cases:
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert q35.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------- the documented loop
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3c", "int8"])
+def test_decode_loop_as_documented(fmt):
+    """prompt -> weights -> eviction -> steps that attend to the current token from its own rows, which stores its weight:
+    what places in key_mass held before plays no part, neither behind an eviction nor in pages of another sequence.  Every
+    step, and a second eviction by the weights that came together, against the oracle on the same state"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, K, W = 16, 2, 4, 64, 90, 8
+    ctxs = [260, 85, 171]
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 58, extra=9)
+    pool = torch.arange(cache.shape[0], dtype=torch.int32)[~torch.isin(torch.arange(cache.shape[0]), table[1].long())].tolist()
+    gc, gs = gpu(cache), gpu_scales(scales)
+    row_scale = gs.get("paged_kv_scale")
+
+    def now():  # what the oracle reads: the GPU's own state
+        return gc.cpu(), {} if row_scale is None else {"row_scale": row_scale.cpu()}
+
+    gm = torch.rand((cache.shape[0], P, HKV), generator=g).mul(1e4).cuda()  # of whoever had the pages before
+    q = q_rows(3 * W, HKV * G, D, g, 2.0)
+    q35.paged_key_mass(gpu(q), gc, gpu(windows([W] * 3)), *gpu(table), gm, **gs)
+    mass = gm.cpu()
+    kept = q35.evict_keys(gc, gm, *gpu(table), K, keep_first=2, keep_last=W, **gs)
+    rk, rc, rm, rs = olc.evict(cache, mass, *table, K, 2, W, scales.get("row_scale"))
+    assert torch.equal(kept.cpu(), rk) and torch.equal(gc.cpu().view(torch.uint8), rc.view(torch.uint8)) and torch.equal(gm.cpu(), rm)
+    ctxs = [min(c, K) for c in ctxs]
+    pages_of = [table[1][int(table[0][b]):int(table[0][b + 1])].tolist()[:-(-ctxs[b] // P)] for b in range(3)]
+    for b in range(3):
+        pool += [p for p in table[1][int(table[0][b]):int(table[0][b + 1])].tolist() if p not in pages_of[b]]
+
+    def listed():
+        return (windows([len(p) for p in pages_of]), torch.tensor(sum(pages_of, []), dtype=torch.int32),
+                torch.tensor([c - (len(p) - 1) * P for c, p in zip(ctxs, pages_of)], dtype=torch.int32))
+
+    bounds = q35.page_key_bounds(gc, *gpu(listed()), paged_kv_scale=row_scale)
+    for step in range(20):
+        t, gt = listed(), gpu(listed())
+        for b in range(3):
+            if ctxs[b] == len(pages_of[b]) * P:
+                pages_of[b].append(pool.pop(0))
+        loc = torch.tensor([[pages_of[b][c // P], c % P] for b, c in enumerate(ctxs)], dtype=torch.int32)
+        kn, vn, qs = q_rows(3, HKV, D, g), q_rows(3, HKV, D, g), q_rows(3, HKV * G, D, g, 2.0)
+        c, s = now()
+        sel = q35.select_pages(gpu(qs), bounds, *gt, 3, keep_first=1, keep_last=1)
+        rb = olc.page_bounds(c, *t, torch.zeros(bounds.shape, dtype=torch.bfloat16), row_scale=s.get("row_scale"))
+        assert torch.equal(sel.cpu(), olc.select_pages(qs, rb, *t, 3, 1, 1))
+        before = gm.cpu()
+        out = q35.paged_attention_sparse(gpu(qs), gc, *gt, sel, key_mass=gm, k_new=gpu(kn), v_new=gpu(vn), cache_location=gpu(loc), **gs)
+        ref, rmass, size, reach = olc.sparse_decode(qs, c, *t, sel.cpu(), before, k_new=kn, v_new=vn, cache_location=loc, **s)
+        check_out(out, ref, size, reach, D, fmt)
+        before[loc[:, 0].long(), loc[:, 1].long()] = 0.0  # stored there
+        check_added(gm, rmass, before, float(reach.max()), D, G)
+        q35.kv_write(gc, gpu(loc), gpu(kn), gpu(vn), paged_kv_scale=row_scale)
+        ctxs = [n + 1 for n in ctxs]
+        q35.page_key_bounds(gc, *gpu(listed()), bounds, first_page=gpu(torch.tensor([len(p) - 1 for p in pages_of], dtype=torch.int32)),
+                            paged_kv_scale=row_scale)
+    (c, s), t, mass = now(), listed(), gm.cpu()
+    kept = q35.evict_keys(gc, gm, *gpu(t), K - 20, keep_first=2, keep_last=4, **gs)
+    assert torch.equal(kept.cpu(), olc.evict(c, mass, *t, K - 20, 2, 4, s.get("row_scale"))[0])
+    page, row = olc._places(*t, P, 0)
+    assert mass[page, row].max() < 40 * G * W  # no place kept what it held in the beginning
+    assert q35.device_status() == 0
