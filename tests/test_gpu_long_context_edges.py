@@ -265,3 +265,258 @@ def test_decode_loop_as_documented(fmt):
     page, row = olc._places(*t, P, 0)
     assert mass[page, row].max() < 40 * G * W  # no place kept what it held in the beginning
     assert q35.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------- added weights, row by row
+@pytest.mark.parametrize("held", [0.0, 1.0])
+@pytest.mark.parametrize("fmt,D,HKV,G,n", [("bf16", 256, 4, 2, 57344), ("int8", 128, 8, 3, 86016), ("e4m3c", 64, 16, 1, 57344)])
+def test_weights_of_many_rows_one_by_one(fmt, D, HKV, G, n, held):
+    """equal shares of all pages: a row's weight is about 1 / n, and every one of them is there, whatever the row held"""
+    import ax_dsl_kernels_b200 as q35
+    ctxs, P = [0, 1, n // 2, 33, n // 2 + 77], 64
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 59, extra=8)
+    q, kn, vn = q_rows(5, HKV * G, D, g, 2.0), q_rows(5, HKV, D, g), q_rows(5, HKV, D, g)
+    spare = torch.arange(cache.shape[0], dtype=torch.int32)[~torch.isin(torch.arange(cache.shape[0]), table[1].long())]
+    loc = torch.stack([spare[:5], torch.arange(5, dtype=torch.int32)], 1).contiguous()
+    old = torch.rand((cache.shape[0], P, HKV), generator=g) * held
+    _, ref, _, reach = olc.sparse_decode(q, cache, *table, None, old, **scales, k_new=kn, v_new=vn, cache_location=loc)
+    gm = gpu(old)
+    q35.paged_attention_sparse(gpu(q), gpu(cache), *gpu(table), key_mass=gm, k_new=gpu(kn), v_new=gpu(vn), cache_location=gpu(loc),
+                               **gpu_scales(scales))
+    old[loc[:, 0].long(), loc[:, 1].long()] = 0.0
+    check_added(gm, ref, old, float(reach.max()), D, G)
+    assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("held", [0.0, 1.0])
+def test_weights_added_to_shared_pages_one_by_one(fmt, held):
+    """six sequences that share their first pages, from windows and from single queries"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, n = 16, 2, 6, 128, 6
+    ctxs = [400 + 37 * i for i in range(n)]
+    cache, (indptr, indices, last), scales, g = make(ctxs, P, HKV, D, fmt, 60)
+    for b in range(1, n):
+        indices[int(indptr[b]):int(indptr[b]) + 20] = indices[:20]
+    table, T = (indptr, indices, last), [1, 30, 0, 60, 25, 130]
+    q, old = q_rows(sum(T), HKV * G, D, g, 2.0), torch.rand((cache.shape[0], P, HKV), generator=g) * held
+    ref, reach = olc.key_mass(q, cache, windows(T), *table, old, accumulate=True, **scales)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows(T)), *gpu(table), gm, accumulate=True, **gpu_scales(scales))
+    check_added(gm, ref, old, reach, D, sum(T) * G, adds=n)
+    q = q_rows(n, HKV * G, D, g, 2.0)
+    _, ref, _, reach = olc.sparse_decode(q, cache, *table, None, old, **scales)
+    gm = gpu(old)
+    q35.paged_attention_sparse(gpu(q), gpu(cache), *gpu(table), key_mass=gm, **gpu_scales(scales))
+    check_added(gm, ref, old, float(reach.max()), D, n * G, adds=n)
+
+
+# ---------------------------------------------------------------------------------------------------- sizes
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("S", [32, 33, 64, 70])
+def test_long_lists_of_chosen_pages(fmt, S):
+    """lists that end inside a warp's 32 entries, at their border, and not at all"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D = 16, 2, 5, 64
+    ctxs = [1200, 16 * 64, 16 * 32, 16 * 33 - 1, 16 * 31, 900, 5]
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 61)
+    cache, _ = poison_behind(cache, table, P)
+    q, old = q_rows(len(ctxs), HKV * G, D, g, 2.0), torch.rand((cache.shape[0], P, HKV), generator=g)
+    pages = random_pages(ctxs, P, HKV, S, g)
+    for b, h, n in ((0, 0, 32), (0, 1, 31), (1, 0, 33), (5, 1, 0)):  # and lists of chosen lengths
+        pages[b, h, min(n, S):] = -1
+    ref, mass, size, reach = olc.sparse_decode(q, cache, *table, pages, old, **scales)
+    gm = gpu(old)
+    out = q35.paged_attention_sparse(gpu(q), gpu(cache), *gpu(table), gpu(pages), key_mass=gm, **gpu_scales(scales))
+    check_out(out, ref, size, reach, D, fmt)
+    check_added(gm, mass, old, float(reach.max()), D, G)
+    assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt,D", [("bf16", 256), ("e4m3", 128), ("int8", 64)])
+def test_one_long_sequence(fmt, D):
+    """the most CTAs to a row, the most ranges of keys to a window; chosen pages as many as there are"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, ctx, T = 64, 2, 4, 20011, 5
+    cache, table, scales, g = make([ctx], P, HKV, D, fmt, 62)
+    cache, _ = poison_behind(cache, table, P)
+    q, old = q_rows(T, HKV * G, D, g, 2.0), torch.rand((cache.shape[0], P, HKV), generator=g)
+    every = torch.arange(-(-ctx // P), dtype=torch.int32).expand(1, HKV, -1).contiguous()
+    ref, mass, size, reach = olc.sparse_decode(q[:1], cache, *table, None, old, **scales)
+    for pages in (None, gpu(every)):
+        gm = gpu(old)
+        out = q35.paged_attention_sparse(gpu(q[:1]), gpu(cache), *gpu(table), pages, key_mass=gm, **gpu_scales(scales))
+        check_out(out, ref, size, reach, D, fmt)
+        check_added(gm, mass, old, float(reach.max()), D, G)
+    ref, reach = olc.key_mass(q, cache, windows([T]), *table, old, **scales)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows([T])), *gpu(table), gm, **gpu_scales(scales))
+    base = old.clone()
+    base[olc._places(*table, P, 0)] = 0.0
+    check_added(gm, ref, base, reach, D, T * G)
+    assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("G", [43, 64, 65, 100, 128])
+def test_key_mass_of_large_head_groups(G):
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, D, ctxs, T = 32, 2, 64, [300, 130, 9], [12, 0, 9]
+    cache, table, _, g = make(ctxs, P, HKV, D, "bf16", 63)
+    q, old = q_rows(sum(T), HKV * G, D, g, 2.0), torch.rand((cache.shape[0], P, HKV), generator=g)
+    ref, reach = olc.key_mass(q, cache, windows(T), *table, old, accumulate=True)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows(T)), *gpu(table), gm, accumulate=True)
+    check_added(gm, ref, old, reach, D, max(T) * G)
+    assert q35.device_status() == 0
+
+
+def test_more_sequences_than_a_warp_has_lanes():
+    """70 sequences: the windows' and the equal shares' search goes around more than twice"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, B = 16, 2, 3, 64, 70
+    g = torch.Generator().manual_seed(64)
+    ctxs = torch.randint(0, 400, (B,), generator=g).tolist()
+    T = [min(c, t) for c, t in zip(ctxs, torch.randint(0, 90, (B,), generator=g).tolist())]
+    cache, table, _, g = make(ctxs, P, HKV, D, "bf16", 65)
+    q, old = q_rows(sum(T), HKV * G, D, g, 2.0), torch.rand((cache.shape[0], P, HKV), generator=g)
+    ref, reach = olc.key_mass(q, cache, windows(T), *table, old, accumulate=True)
+    gm = gpu(old)
+    q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows(T)), *gpu(table), gm, accumulate=True)
+    check_added(gm, ref, old, reach, D, max(T) * G)
+    # equal shares: against every sequence by itself
+    HKV, B = 16, 40
+    ctxs = [0 if b % 9 == 4 else 9000 + 53 * b for b in range(B)]
+    n = [-(-c // 64) for c in ctxs]
+    cache = torch.randn((sum(n), 2, 64, HKV, D), device="cuda").to(torch.bfloat16)
+    q = gpu(q_rows(B, HKV, D, g, 2.0))
+    indptr, indices = gpu(windows(n)), torch.randperm(sum(n), device="cuda").to(torch.int32)
+    last = gpu(torch.tensor([c - (m - 1) * 64 if m else 0 for c, m in zip(ctxs, n)], dtype=torch.int32))
+    gm = torch.zeros((sum(n), 64, HKV), device="cuda")
+    out = q35.paged_attention_sparse(q, cache, indptr, indices, last, key_mass=gm)
+    one, gn = torch.empty_like(out), torch.zeros_like(gm)
+    for b in range(B):
+        lo, hi = sum(n[:b]), sum(n[:b + 1])
+        q35.paged_attention_sparse(q[b:b + 1], cache, indptr[b:b + 2] - lo, indices[lo:hi].clone(), last[b:b + 1], out=one[b:b + 1],
+                                   key_mass=gn)
+    # two evaluations of scores with R <= 20 here (|q| |k| scale is 10 on average): weights differ by twice 2 (D + 4) 2^-23 R
+    # < 2^-10 of themselves at most, outputs by that of sum p |v| < 1 and one step of bf16
+    assert ((out.float() - one.float()).abs() <= one.float().abs() * 2.0 ** -7 + 2.0 ** -10).all()
+    assert (out[4] == 0).all() and ((gm - gn).abs() <= gn * 2.0 ** -10).all()
+    assert torch.allclose(gm.double().sum(), torch.tensor(float(HKV * (B - 4)), dtype=torch.float64, device="cuda"), rtol=2.0 ** -12)
+    assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 1.5])
+def test_other_scales(scale):
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, ctxs, T = 64, 2, 6, 64, [500, 200], [70, 3]
+    cache, table, _, g = make(ctxs, P, HKV, D, "bf16", 66)
+    q, old = q_rows(sum(T), HKV * G, D, g), torch.rand((cache.shape[0], P, HKV), generator=g)
+    for s in (scale, torch.tensor([scale], device="cuda")):
+        ref, _ = olc.key_mass(q, cache, windows(T), *table, old, accumulate=True, sm_scale=scale)
+        _, reach = olc.key_mass(q, cache, windows(T), *table, old, sm_scale=abs(scale))
+        gm = gpu(old)
+        q35.paged_key_mass(gpu(q), gpu(cache), gpu(windows(T)), *gpu(table), gm, accumulate=True, sm_scale=s)
+        check_added(gm, ref, old, reach, D, max(T) * G)
+        ref, mass, size, _ = olc.sparse_decode(q[:2], cache, *table, None, old, sm_scale=scale)
+        _, _, _, reach = olc.sparse_decode(q[:2], cache, *table, sm_scale=abs(scale))
+        gm = gpu(old)
+        out = q35.paged_attention_sparse(gpu(q[:2]), gpu(cache), *gpu(table), key_mass=gm, sm_scale=s)
+        check_out(out, ref, size, reach, D)
+        check_added(gm, mass, old, float(reach.max()), D, G)
+
+
+@pytest.mark.parametrize("fmt,D", [("bf16", 32), ("bf16", 96), ("bf16", 160), ("int8", 192), ("int8", 320), ("bf16", 512), ("bf16", 1024)])
+@pytest.mark.parametrize("B,K", [(1, 600), (5, 100), (90, 130)])
+def test_evict_rows_of_other_widths(fmt, D, B, K):
+    """rows of 64 to 2048 bytes, among them those whose pieces do not divide a warp: K and V by a cluster each, by one, by
+    one CTA"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV = 16, 2
+    ctxs = [700, 0, 130, 101, 1][:B] if B <= 5 else [(37 * i) % 200 for i in range(B)]
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 67)
+    mass = torch.randn((cache.shape[0], P, HKV), generator=g).mul(2).exp()
+    ref, rcache, rmass, rrs = olc.evict(cache, mass, *table, K, 2, 9, scales.get("row_scale"))
+    gc, gm, gs = gpu(cache), gpu(mass), gpu_scales(scales)
+    kept = q35.evict_keys(gc, gm, *gpu(table), K, keep_first=2, keep_last=9, **gs)
+    assert torch.equal(kept.cpu(), ref)
+    assert torch.equal(gc.cpu().view(torch.uint8), rcache.view(torch.uint8)) and torch.equal(gm.cpu(), rmass)
+    assert rrs is None or torch.equal(gs["paged_kv_scale"].cpu(), rrs)
+    assert q35.device_status() == 0
+
+
+def test_select_pages_of_more_than_fit_on_chip():
+    """sequences of more than 16384 pages beside shorter ones; pages that differ, and pages that are all the same"""
+    import ax_dsl_kernels_b200 as q35
+    from test_gpu_long_context import select_case
+    q, bounds, table = select_case([20000, 300, 16384, 17003], 2, 64, 2, 68)
+    same = bounds.clone()
+    same[table[1].long()] = bounds[table[1][0].long()]
+    for b in (bounds, same):
+        for S, first, last in ((100, 1, 2), (16500, 0, 1)):
+            ref = olc.select_pages(q, b, *table, S, first, last)
+            got = q35.select_pages(gpu(q), gpu(b), *gpu(table), S, keep_first=first, keep_last=last)
+            assert torch.equal(got.cpu(), ref)
+    assert q35.device_status() == 0
+
+
+def test_nothing_cached_and_no_queries():
+    """tables without an entry, sequences without a row, a window of no tokens, no sequence at all"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D = 16, 2, 4, 64
+    cache, _, _, g = make([], P, HKV, D, "bf16", 69)
+    gc, gm = gpu(cache), torch.full((cache.shape[0], P, HKV), 3.0, device="cuda")
+    for B in (0, 2):
+        t = gpu((torch.zeros(B + 1, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(B, dtype=torch.int32)))
+        q = gpu(q_rows(B, HKV * G, D, g))
+        bounds = q35.page_key_bounds(gc, *t)
+        assert (bounds == 0).all()
+        assert (q35.select_pages(q, bounds, *t, 3, keep_first=1) == -1).all()
+        for pages in (None, torch.full((B, HKV, 3), -1, dtype=torch.int32, device="cuda")):
+            assert (q35.paged_attention_sparse(q, gc, *t, pages, key_mass=gm) == 0).all()
+        q35.paged_key_mass(gpu(q_rows(0, HKV * G, D, g)), gc, torch.zeros(B + 1, dtype=torch.int32, device="cuda"), *t, gm)
+        assert (q35.evict_keys(gc, gm, *t, 5, keep_last=2) == -1).all()
+        assert (gm == 3.0).all() and torch.equal(gc.cpu(), cache)
+    cache, table, _, g = make([40, 0, 20], P, HKV, D, "bf16", 70)  # rows, but no window: nobody gave them a weight
+    gm = torch.full((cache.shape[0], P, HKV), 3.0, device="cuda")
+    q35.paged_key_mass(gpu(q_rows(0, HKV * G, D, g)), gpu(cache), torch.zeros(4, dtype=torch.int32, device="cuda"), *gpu(table), gm)
+    ref, _ = olc.key_mass(q_rows(0, HKV * G, D, g), cache, torch.zeros(4, dtype=torch.int32), *table, torch.full(gm.shape, 3.0))
+    assert torch.equal(gm.cpu().double(), ref) and (ref == 0).sum() == 60 * HKV
+    assert q35.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3c", "int8"])
+def test_pages_far_into_a_large_cache(fmt):
+    """the same rows in the last pages of a cache whose elements and bytes pass 2^31 and 2^32: the same results"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D, total = 64, 2, 8, 256, 40000 if fmt == "bf16" else 70000
+    ctxs, T = [900, 300, 65], [40, 3, 0]
+    cache, table, scales, g = make(ctxs, P, HKV, D, fmt, 71)
+    n = cache.shape[0]
+    far = torch.arange(total - n, total, device="cuda")
+    big = torch.empty((total, 2, P, HKV, D), dtype=torch.uint8 if fmt != "bf16" else torch.bfloat16, device="cuda")
+    assert big.numel() > 2 ** 31 and big.numel() * big.element_size() > 2 ** 32
+    big[far] = gpu(cache) if fmt == "bf16" else gpu(cache).view(torch.uint8)
+    big = big if fmt == "bf16" else big.view(cache.dtype)
+    mass = torch.rand((n, P, HKV), generator=g)
+    qs, qw = gpu(q_rows(3, HKV * G, D, g, 2.0)), gpu(q_rows(sum(T), HKV * G, D, g, 2.0))
+    results = []
+    for c, shift in ((gpu(cache), 0), (big, total - n)):
+        pages = c.shape[0]
+        t = (gpu(table[0]), gpu(table[1]) + shift, gpu(table[2]))
+        gm = torch.zeros((pages, P, HKV), device="cuda")
+        gm[shift:shift + n] = gpu(mass)
+        s = {}
+        if "row_scale" in scales:
+            s["paged_kv_scale"] = torch.zeros((pages, 2, P, HKV), dtype=torch.bfloat16, device="cuda")
+            s["paged_kv_scale"][shift:shift + n] = gpu(scales["row_scale"])
+        bounds = q35.page_key_bounds(c, *t, **s)
+        sel = q35.select_pages(qs, bounds, *t, 4)
+        out = q35.paged_attention_sparse(qs, c, *t, sel, key_mass=gm, **s)
+        q35.paged_key_mass(qw, c, gpu(windows(T)), *t, gm, accumulate=True, **s)
+        kept = q35.evict_keys(c, gm, *t, 200, keep_last=5, **s)
+        results.append([x[shift:shift + n] if x.shape[0] == pages else x for x in (
+            bounds, sel, out, gm, kept, c.view(torch.uint8) if fmt != "bf16" else c, *s.values())])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert q35.device_status() == 0
