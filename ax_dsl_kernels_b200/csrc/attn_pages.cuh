@@ -84,8 +84,9 @@ __device__ __forceinline__ int2 find_item(int B, int index, Count count) {
     }
     const unsigned hit = __ballot_sync(0xffffffffu, before + inc > index);
     if (hit) {
-      const int l = __ffs(hit) - 1;
-      return make_int2(b0 + l, index - before - __shfl_sync(0xffffffffu, inc - c, l));
+      const int l = __ffs(hit) - 1, at = index - before - __shfl_sync(0xffffffffu, inc - c, l);
+      // ranges of a bad table may overlap, and the counts of a warp's sequences then wrap around: no item
+      return unsigned(at) < unsigned(__shfl_sync(0xffffffffu, c, l)) ? make_int2(b0 + l, at) : make_int2(-1, 0);
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
   }

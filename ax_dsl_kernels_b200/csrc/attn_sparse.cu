@@ -691,8 +691,9 @@ __global__ void __launch_bounds__(256) sparse_merge_kernel(const SparseArgs a) {
     if (lane == 0) s_new[warp] = dot * scale_log2;
   }
   __syncthreads();
-  const int first = s_flat[1] / s_flat[0];
-  const int n = steps ? min(a.n_cta, (s_flat[1] + steps - 1) / s_flat[0] - first + 1) : 0;
+  // (held to the CTAs there are: ranges of a bad table may overlap and add up to more steps than an int holds)
+  const int first = min(max(s_flat[1] / s_flat[0], 0), a.n_cta - 1);
+  const int n = steps ? min(max((s_flat[1] + steps - 1) / s_flat[0] - first + 1, 0), a.n_cta - first) : 0;
   const float* ml = a.part_ml + size_t(row + first) * (2 * SP_G);
   {
     const int g = tid % SP_G, j0 = tid / SP_G;
