@@ -244,11 +244,13 @@ constexpr int SEL_ZONE = 512;      // undecided pages that stay in shared memory
 // pages of sequence b that hold a row, without knowing P
 __device__ __forceinline__ int2 select_range(const SelectArgs& a, int b) {
   const int lo = a.t.indptr[b], hi = a.t.indptr[b + 1];
-  if (lo < 0 || hi < lo || hi > a.t.n_indices) {
+  const bool range = lo >= 0 && hi >= lo && hi <= a.t.n_indices;
+  const int last = range && hi > lo ? a.t.last_page_len[b] : 0;
+  if (!range || last < 0) {
     atomicOr(a.t.status, DS_BAD_PAGE);
     return make_int2(0, 0);
   }
-  return make_int2(lo, hi - lo - (hi > lo && a.t.last_page_len[b] <= 0 ? 1 : 0));
+  return make_int2(lo, hi - lo - (hi > lo && last == 0 ? 1 : 0));
 }
 __device__ __forceinline__ uint32_t pos_pair(uint32_t x) {
   __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f));

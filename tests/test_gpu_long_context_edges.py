@@ -520,3 +520,29 @@ def test_pages_far_into_a_large_cache(fmt):
     for a, b in zip(*results):
         assert torch.equal(a, b)
     assert q35.device_status() == 0
+
+
+def test_last_pages_of_negative_length():
+    """every role records one and takes the sequence for empty"""
+    import ax_dsl_kernels_b200 as q35
+    P, HKV, G, D = 16, 2, 4, 64
+    cache, table, _, g = make([100, 60], P, HKV, D, "bf16", 72)
+    q, mass = gpu(q_rows(2, HKV * G, D, g)), torch.rand((cache.shape[0], P, HKV), generator=g)
+    fine = gpu(table)
+    bounds = q35.page_key_bounds(gpu(cache), *fine)
+    want = q35.select_pages(q, bounds, *fine, 3), q35.paged_attention_sparse(q, gpu(cache), *fine)
+    t = (fine[0], fine[1], torch.tensor([-1, int(table[2][1])], dtype=torch.int32, device="cuda"))
+    gc, gm = gpu(cache), gpu(mass)
+    assert q35.device_status() == 0
+    got = q35.select_pages(q, bounds, *t, 3)
+    assert q35.device_status() & 1 and (got[0] == -1).all() and torch.equal(got[1], want[0][1])
+    got = q35.paged_attention_sparse(q, gc, *t)
+    assert q35.device_status() & 1 and (got[0] == 0).all() and torch.equal(got[1], want[1][1])
+    q35.page_key_bounds(gc, *t, bounds.clone())
+    assert q35.device_status() & 1
+    q35.paged_key_mass(q, gc, gpu(windows([0, 2])), *t, gm)
+    assert q35.device_status() & 1
+    page, row = olc._places(*table, P, 0)
+    assert torch.equal(gm.cpu()[page, row], mass[page, row])
+    assert (q35.evict_keys(gc, gm, *t, 10)[0] == -1).all() and q35.device_status() & 1
+    assert torch.equal(gc.cpu()[page, :, row], cache[page, :, row]) and torch.equal(gm.cpu()[page, row], mass[page, row])
