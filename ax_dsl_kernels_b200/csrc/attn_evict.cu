@@ -11,7 +11,7 @@
 // only have to wait until the whole cluster has loaded that round.  A warp owns whole rows of a round: cp.async brings
 // them into its part of the shared memory, and it stores them from there while the cluster's barrier for the next round
 // closes and the one after that is on its way.  (An SM stores 27 bytes a cycle here; loads and barriers hide behind it.)
-// (Choice and moves, 32 x 4000 of up to 16384 bf16 rows: one CTA per 64-byte column slice, without clusters, 175 us; this
+// (Choice and moves, 32 x 4000 of up to 16384 bf16 rows, calls among others: one CTA per 64-byte column slice, without clusters, 175 us; this
 // 50, with a choice by one CTA per row 60.  115 MB read and written take 35 us at HBM's rate.  One bulk copy per row and
 // direction instead of cp.async and stores: as long.)
 #include <cooperative_groups.h>

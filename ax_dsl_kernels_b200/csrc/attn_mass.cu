@@ -16,9 +16,10 @@
 // thread owns a key and adds up exp2(s - lse).  So every reduction runs along a thread's own columns, every sum has one
 // owner and a fixed order, and nothing is exchanged but the groups' partial sums.
 // The groups' arithmetic is what takes longest to keep up: four warps per scheduler hide its latency, two numbers go to
-// an fma or add (f32x2), tiles that every row sees whole have a path without a mask.  (Two groups, a mask for every
-// tile, one number at a time: 273 us instead of 245 for 2047 queries over 8192 rows.  The held operand in tensor memory
-// and three groups: 239, but 44 instead of 37 for 32 queries over four prompts, whose one load per item it exposes.)
+// an fma or add (f32x2), tiles that every row sees whole have a path without a mask.  (Graph replays of one
+// input.  Two groups, a mask for every tile, one number at a time: 273 us instead of 245 for 2047 queries over 8192 rows.
+// The held operand in tensor memory and three groups: 239, but 44 instead of 37 for 32 queries over four prompts at a tile
+// per CTA in pass 2, whose one load per item it exposes.  Several tiles per CTA have since made 30 of the 37.)
 //
 // A block holds the (token, head) pairs of floor(128 / G) tokens, fetched as one 3-D box; the keys come straight from the
 // pages where the cache is bf16 and its pages hold whole swizzle atoms (8 rows), else from a bf16 copy made first.
@@ -588,8 +589,8 @@ static int launch_mass(const MassArgs& a, const CUtensorMap& qmap, const CUtenso
   }
   // Short windows: a CTA per SM takes its tiles one after the other, so that what a tile waits for (tables, first loads,
   // the last exponentials) is met while its neighbours work.  Long ones, 32 blocks of queries and more: a CTA per tile, so
-  // that the lengths even out (four prompts of up to 8192, 2 heads: 32 queries 29.8 us and 37.2, 300 queries 118 and 123;
-  // 2047 queries 646 and 620).
+  // that the lengths even out (graph replays, four prompts of up to 8192, 2 heads: 32 queries 29.8 us and 37.2, 300
+  // queries 118 and 123; 2047 queries 646 and 620).
   int64_t grid = tiles * a.HKV;
   if (grid > sm_count() && blocks <= 32 * int64_t(a.t.B)) {
     const int64_t least = (grid + KM_ITEMS - 1) / KM_ITEMS;

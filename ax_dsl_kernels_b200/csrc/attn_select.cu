@@ -212,13 +212,15 @@ int run_attn_page_bounds(Call& c) {
 // pages.  So the scores are found twice: sum_d max(q_d lo_d, q_d hi_d) = max(q, 0) . hi + min(q, 0) . lo is a product
 // of bf16 rows that the tensor cores do for all heads at once in fp32, with an error of at most n 2^-23 sum |terms| for
 // any order of n = 2 D terms, and a third product, |q| . max(|lo|, |hi|), bounds that sum; the few pages within that
-// error of the border (most often one to three) are scored again in fp64, where the sum of 512 products of 16
-// significant bits is as good as exact.  (An infinite bound turns 0 * inf of the split form into a NaN and the error
-// into infinity: then every page is scored again, by the definition.)
+// error of the border (most often one to three) are scored again in fp64: a sum of 256 products of 16 significant bits is
+// exact there while they lie within 2^28 of one another, else rounded at 2^-53 of its largest partial sum.  (An infinite
+// bound turns 0 * inf of the split form into a NaN and the error into infinity: then every page is scored again, by the
+// definition.)
 //
 // Bound: HBM for the bounds (each read once); at one sequence the chain of the selection.  One launch: a cluster of up
 // to 8 CTAs scores the pages of one (sequence, KV head) and leaves the scores in the shared memory of its first CTA,
-// which chooses (two kernels with the scores in HBM between them: 21.6 us instead of 10.0 for 256 pages, 31.8 instead of 18.0 for 32 rows of 2048).
+// which chooses (two kernels with the scores in HBM between them, graph replays with the bounds in L2: 21.6 us instead of
+// 10.0 for 256 pages, 31.8 instead of 18.0 for 32 rows of 2048).
 struct SelectArgs {
   const __nv_bfloat16* q;       // [B, HQ, D]
   const __nv_bfloat16* bounds;  // [pages, 2, HKV, D]
@@ -669,7 +671,8 @@ int run_attn_select_pages(Call& c) {
   a.zone = reinterpret_cast<int*>(w + o_zone);
   a.score = reinterpret_cast<float*>(w + o_sc); a.flag = w + o_flag;
   // four 16-page tiles per CTA for the average sequence (an SM reads a quarter of a megabyte in 3 us), as far as all
-  // clusters run at once, one CTA to an SM (clusters of 8 that have to share SMs do not all find a place: 32 rows of 2048 pages 25.4 us with 4, 28.9 with 8)
+  // clusters run at once, one CTA to an SM (clusters of 8 that have to share SMs do not all find a place: 32 rows of 2048
+  // pages, bounds from HBM, 25.4 us with 4, 28.9 with 8)
   const int64_t tiles = ((a.t.n_indices + B - 1) / B + 15) / 16;
   int cluster = 1;
   while (cluster < 8 && cluster * 4 < tiles && B * HKV * cluster * 2 <= sm_count()) cluster *= 2;

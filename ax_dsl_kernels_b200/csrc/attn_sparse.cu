@@ -7,9 +7,11 @@
 // Bound: HBM, K and V of the chosen rows once.  A cluster of C CTAs serves one (sequence, KV head): its chosen rows,
 // laid end to end, are cut into C contiguous ranges, every CTA runs one pass with a running maximum and sum over its
 // range, and the C partial results are merged through distributed shared memory -- one launch, no partials in HBM, no
-// counters.  (All pages of many long rows: the flat form, equal shares per CTA and a second kernel that merges.)  Inside a CTA each warp takes steps of 32 rows through its own cp.async ring (16-byte chunks, XOR-swizzled
-// rows), with no block barrier in the loop.  Scores are computed transposed (S^T = K Q^T, mma.m16n8k16) so that the up
-// to 8 query heads of a KV head are the n = 8 side and O^T takes D / 4 registers a lane.
+// counters.  (All pages of many long rows: the flat form, equal shares per CTA and a second kernel that merges.)  Inside a
+// CTA each warp takes steps of 32 rows through its own cp.async ring (16-byte chunks, XOR-swizzled rows), with no block
+// barrier in the loop.  Scores are computed transposed (S^T = K Q^T, mma.m16n8k16) so that the up to 8 query heads of a KV
+// head are the n = 8 side and O^T takes D / 4 registers a lane.  (Times here are graph replays, but for those of weights
+// and sums, which are calls among others.)
 //
 // The weights need the final M and L, so each CTA parks its scores (fp32, 32 bytes per row against 4 D of K and V) in
 // the workspace and turns them into weights after the merge; a row's weights are added by the one CTA that read it.
@@ -746,8 +748,8 @@ __global__ void __launch_bounds__(256) sparse_merge_kernel(const SparseArgs a) {
 
 // CTAs per (sequence, KV head).  `slots` CTAs are resident at a time.
 // Chosen pages: all rows of the grid have about the same length, the most CTAs that still run at once (64 sequences x
-// 2 heads x 4096 rows on 148 slots: 1 CTA 92 us, 2: 95, 4: 112).  All pages: lengths differ, so at least one CTA per
-// slot, and more to even them out (32 x 4 ragged E4M3 rows on 296 slots: 2 CTAs 65 us, 4: 60, 8: 76).
+// 2 heads x 4096 rows on 148 slots: 1 CTA 90 us, 2: 98, 4: 113).  All pages: lengths differ, so at least one CTA per
+// slot, and more to even them out (32 x 4 ragged E4M3 rows with weights on 296 slots: 2 CTAs 59 us, 4: 54, 8: 70).
 // Never more than one step per warp; 16 (beyond the portable 8) for a few long rows.
 static int sparse_cluster(int64_t rows, int64_t steps, int slots, bool chosen) {
   int c = 1;
@@ -837,9 +839,11 @@ int run_attn_sparse_decode(Call& c) {
   Q35_REQUIRE(S <= INT_MAX / 2 / P && B * HKV <= INT_MAX / 16, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);
   const int64_t rows = pages.present ? B * HKV * S * P : HKV * int64_t(a.t.n_indices) * P;
   // The flat form, for all pages of many rows: every CTA the same number of steps, whatever the lengths, a second kernel
-  // that merges.  It pays from 48 steps per CTA and 256 per row on (8 rows of 60000 bf16: 92 us, clusters 135; 74 rows of
-  // 32000 E4M3: 207 and 281; but 128 ragged rows of 73 steps: 85 and 72); below, and for chosen pages, whose rows are
-  // about equally long, one launch of clusters.
+  // that merges.  It pays from 48 steps per CTA and 256 per row on (8 rows of 60000 bf16: 92 us, clusters 146; 74 rows of
+  // 32000 E4M3: 203 and 308; but 128 ragged E4M3 rows of up to 131 steps, with weights: 60 and 54); below, and for chosen
+  // pages, whose rows are about equally long, one launch of clusters.  Rows too few to fill the GPU's steps stay with the
+  // clusters as well, although equal shares serve them better from about 32000 cached rows on (one sequence of two heads,
+  // 65536 bf16 rows: 43 us, clusters 78; 131072 E4M3 rows: 47 and 133; 16384: 26 and 26, 23 and 24).
   a.n_cta = sm_count() * (D == 256 ? (kv.fmt ? 2 : 1) : D == 128 ? (kv.fmt ? 3 : 2) : 4);
   const int64_t all_steps = HKV * (int64_t(a.t.n_indices) * P / SP_KEYS);
   Q35_REQUIRE(pages.present || all_steps + B * HKV <= INT_MAX, Q35_ERR_UNSUPPORTED, "%s: sizes beyond 32 bits", role);

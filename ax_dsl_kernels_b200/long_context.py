@@ -66,8 +66,8 @@ def select_pages(q, page_bounds, indptr, indices, last_page_len, n_select, out=N
     """The n_select pages of every (sequence, KV head) to attend to: [B, HKV, n_select] int32 positions in the
     sequence's page list (not page ids), ascending, -1 behind when it has fewer.  A page scores
     max over the KV head's query heads of sum_d max(q_d * min_d, q_d * max_d), the most any of its keys can score;
-    ties go to the lower position, a NaN ranks last.  The keep_first first and the keep_last last pages are chosen
-    whatever they score (keep_last before keep_first when they do not all fit).  q [B, HQ, D] bf16."""
+    pages are ordered by these sums in fp64, ties go to the lower position, a NaN ranks last.  The keep_first first and the
+    keep_last last pages are chosen whatever they score (keep_last before keep_first when they do not all fit).  q [B, HQ, D] bf16."""
     if out is None:
         out = torch.empty((q.shape[0], page_bounds.shape[2], int(n_select)), dtype=torch.int32, device=q.device)
     elif out.shape[-1] != n_select:
@@ -89,7 +89,8 @@ def paged_attention_sparse(q, paged_kv_cache, indptr, indices, last_page_len, pa
     (stored, not added: the row is new; the table does not hold it yet).  Without them, a row that is new in the table
     starts from whatever its place in key_mass held -- after an eviction or in a page used again, another row's weight --
     and the caller clears it first.  Unlike paged_attention_decode nothing is written into the cache.
-    A row without any page and without a current token gives zeros.  At most 8 query heads per KV head, head_dim 64, 128
+    A row without any page and without a current token gives zeros; a NaN or an infinity in an attended row of V gives NaN.
+    At most 8 query heads per KV head, head_dim 64, 128
     or 256, page size a multiple of 16.  Formats and scales as in paged_attention_decode."""
     out = torch.empty_like(q) if out is None else out
     kw = dict(q=q, paged_kv_cache=paged_kv_cache, indptr=indptr, indices=indices, last_page_len=last_page_len, out=out)
